@@ -1,4 +1,4 @@
-"""ctypes bindings of the C ABI in include/wick_hip.h, wick_hip_model.h and wick_hip_sampler.h.
+"""ctypes bindings of the C ABI in include/wick_hip.h and the other headers beside it.
 
 This is the binding a host program writes for the library (the Rust side would
 declare the same symbols in an `extern "C"` block).  There is no fallback: if
@@ -58,6 +58,23 @@ SIGNATURES = {
     "wick_hip_sampler_sample": (_I, [_P, _P, _P, _I, _P]),
     "wick_hip_sampler_rng_state": (_I, [_P, _P]),
     "wick_hip_sampler_last_candidates": (_I, [_P, _P, _P, _P, _P, _I]),
+    # wick_hip_batch.h
+    "wick_hip_batch_create": (_I, [_P, ctypes.POINTER(_P)]),
+    "wick_hip_batch_destroy": (None, [_P]),
+    "wick_hip_batch_load_prefix": (_I, [_P, _P, _I]),
+    "wick_hip_batch_write_prefix_device": (_I, [_P, _I, _I, _I, _P, _P]),
+    "wick_hip_batch_plan": (_I, [_P, _P, _P, _I]),
+    "wick_hip_batch_shape": (_I, [_P]),
+    "wick_hip_batch_append_device": (_I, [_P, _I, _P, _P]),
+    "wick_hip_batch_attention_device": (_I, [_P, _I, _P, _P]),
+    "wick_hip_batch_append": (_I, [_P, _I, _P, _P]),
+    "wick_hip_batch_attention": (_I, [_P, _I, _P, _P]),
+    "wick_hip_batch_read": (_I, [_P, _I, _I, _I, _I, _P, _P]),
+    "wick_hip_batch_set_stream": (_I, [_P, _P]),
+    "wick_hip_batch_synchronize": (_I, [_P]),
+    "wick_hip_batch_scratch_bytes": (ctypes.c_longlong, [_P]),
+    # wick_hip_logits.h
+    "wick_hip_logits_adjust_device": (_I, [_P, _P, _I, _I, _I, _P, _I, _P]),
 }
 
 _lib = None

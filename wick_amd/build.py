@@ -36,9 +36,13 @@ HIP_SOURCES = (
     "wick_amd/csrc/prep.hip",
     "wick_amd/csrc/model.hip",
     "wick_amd/csrc/sampler.hip",
+    "wick_amd/csrc/batch.hip",
+    "wick_amd/csrc/logits.hip",
     "wick_amd/csrc/api.cpp",
     "wick_amd/csrc/model_api.cpp",
     "wick_amd/csrc/sampler_api.cpp",
+    "wick_amd/csrc/batch_api.cpp",
+    "wick_amd/csrc/logits_api.cpp",
 )
 
 

@@ -517,6 +517,12 @@ bool kv_info(const wick_hip_kv *kv, KvInfo *out) {
     return true;
 }
 
+void kv_layer(const wick_hip_kv *kv, int layer, const float **k, const float **v, int *device) {
+    *k = kv->k_layer(layer);
+    *v = kv->v_layer(layer);
+    *device = kv->device;
+}
+
 }  // namespace wick
 
 extern "C" {

@@ -152,6 +152,8 @@ struct KvInfo {
     hipStream_t stream;
 };
 bool kv_info(const wick_hip_kv *kv, KvInfo *out);
+// The K and V arrays of one layer, [kv_heads][capacity][head_dim], and their device.
+void kv_layer(const wick_hip_kv *kv, int layer, const float **k, const float **v, int *device);
 
 // src/model.rs:464-485 for one layer on device arrays, as wick_hip_attend_device
 // except that q_dev is scratch (its contents afterwards are unspecified): for

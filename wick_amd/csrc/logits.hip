@@ -1,0 +1,130 @@
+// logits.hip -- the rules of include/wick_hip_logits.h in one pass over the logits.
+//
+// A workgroup has one row's ids [s0, s0 + SLAB).  It requests its logits and mask words,
+// counts the row's tokens that fall into its slab in LDS (integer adds: any order gives
+// the same counts), notes each id's last bias there, then writes its part of the row.  A
+// row's tokens are read once per slab, from the L2.
+//
+// Bound: HBM, 8 bytes a logit and a mask bit.
+#include <hip/hip_runtime.h>
+
+#include "logits_kernels.h"
+
+namespace wick {
+namespace {
+
+constexpr int kT = 256;
+constexpr uint32_t kSeen = 0x80000000u;
+
+// rows of any alignment: 4 values, aligned as one
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+template <int SLAB>
+__global__ __launch_bounds__(kT) void logits_kernel(LogitArgs a) {
+#pragma clang fp contract(off)
+    constexpr int U = SLAB / (4 * kT);  // passes of 4 ids a thread
+    __shared__ uint32_t count[SLAB];    // times among the generated tokens, and kSeen
+    __shared__ uint32_t bias[SLAB];     // 1 + the number of the id's last bias entry
+    const int tid = threadIdx.x, row = blockIdx.x / a.slabs, s0 = (blockIdx.x - row * a.slabs) * SLAB;
+    const wick_hip_logit_rules &r = a.r;
+    const float *x = a.x + (size_t)row * a.stride;
+    float *out = a.out + (size_t)row * a.out_stride;
+
+    const int words = (a.vocab + 31) / 32;
+    const uint32_t *mask = nullptr;
+    if (r.mask) {
+        const int m = r.mask_row ? r.mask_row[row] : row;
+        if (m >= 0 && m < r.masks) mask = r.mask + (size_t)m * words;
+    }
+    float v[U][4];
+    uint32_t allowed[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int i = s0 + 4 * (tid + u * kT);
+        if (i + 4 <= a.vocab) {
+            const f4u y = *reinterpret_cast<const f4u *>(x + i);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[u][j] = y[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[u][j] = i + j < a.vocab ? x[i + j] : 0.0f;
+        }
+        allowed[u] = ~0u;
+        if (mask && i < a.vocab) allowed[u] = mask[i >> 5] >> (i & 31);
+    }
+
+    int n = r.tokens ? min(max(r.n_tokens[row], 0), r.tokens_stride) : 0;
+    const int prompt = n && r.n_prompt ? r.n_prompt[row] : 0;
+    int b0 = 0, b1 = 0;
+    if (r.bias) {
+        b0 = min(max(r.bias_start[row], 0), r.n_bias);
+        b1 = min(max(r.bias_start[row + 1], 0), r.n_bias);
+    }
+    const bool rules = n > 0 || b1 > b0;
+    if (rules) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            reinterpret_cast<u4 *>(count)[tid + u * kT] = u4{0, 0, 0, 0};
+            reinterpret_cast<u4 *>(bias)[tid + u * kT] = u4{0, 0, 0, 0};
+        }
+        __syncthreads();
+        const uint32_t *tokens = r.tokens + (size_t)row * r.tokens_stride;
+        for (int i = tid; i < n; i += kT) {
+            const uint32_t at = tokens[i] - (uint32_t)s0;
+            if (at < (uint32_t)SLAB) {
+                atomicOr(&count[at], kSeen);
+                if (i >= prompt) atomicAdd(&count[at], 1u);
+            }
+        }
+        for (int i = b0 + tid; i < b1; i += kT) {
+            const uint32_t at = r.bias_ids[i] - (uint32_t)s0;
+            if (at < (uint32_t)SLAB) atomicMax(&bias[at], (uint32_t)(i - b0) + 1);
+        }
+        __syncthreads();
+        const float rep = r.repetition ? r.repetition[row] : 1.0f, pres = r.presence ? r.presence[row] : 0.0f,
+                    freq = r.frequency ? r.frequency[row] : 0.0f;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const u4 c = reinterpret_cast<const u4 *>(count)[tid + u * kT], b = reinterpret_cast<const u4 *>(bias)[tid + u * kT];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float y = v[u][j];
+                if (c[j]) y = y > 0.0f ? y / rep : y * rep;
+                const uint32_t times = c[j] & ~kSeen;
+                if (times) y -= freq * (float)times + pres;
+                if (b[j]) y += r.bias[b0 + b[j] - 1];
+                v[u][j] = y;
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int i = s0 + 4 * (tid + u * kT);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (!(allowed[u] >> j & 1)) v[u][j] = -INFINITY;
+        if (i + 4 <= a.vocab) {
+            *reinterpret_cast<f4u *>(out + i) = f4u{v[u][0], v[u][1], v[u][2], v[u][3]};
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (i + j < a.vocab) out[i + j] = v[u][j];
+        }
+    }
+}
+
+}  // namespace
+
+int logit_slab(int rows, int vocab) { return (long long)rows * ((vocab + 4095) / 4096) >= 256 ? 4096 : 1024; }
+
+hipError_t launch_logits(const LogitArgs &a, hipStream_t s) {
+    const int grid = a.rows * a.slabs;
+    if (logit_slab(a.rows, a.vocab) == 4096)
+        logits_kernel<4096><<<grid, kT, 0, s>>>(a);
+    else
+        logits_kernel<1024><<<grid, kT, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+}  // namespace wick
