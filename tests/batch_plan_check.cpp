@@ -37,12 +37,14 @@ static int check(const BatchLimits &c, const std::vector<int> &start, const std:
     std::vector<int> direct(rows, 0);
     std::map<int, std::vector<int>> of_row;
     for (const BatchItem &it : p.items) {
-        if (it.nrows < 1 || it.nrows > kBatchRows || it.row0 < 0) return bad("item rows", k);
+        if (it.nrows < 1 || it.nrows > kBatchWide || it.row0 < 0) return bad("item rows", k);
         if (it.p0 < 0 || it.p1 > prefix || it.p0 > it.p1 || it.o0 < 0 || it.o0 > it.o1) return bad("item keys", k);
         if (it.seq < 0 && it.o0 != it.o1) return bad("own keys without a sequence", k);
         if (it.seq >= 0 && it.o1 > start[it.seq] + t[it.seq]) return bad("own keys past the end", k);
         for (int r = 0; r < it.nrows; r++) {
-            const int row = it.row0 + r, tok = it.seq < 0 ? p.tokens[row / c.group].split : row / c.group;
+            const int row = it.row0 + r, tok = it.seq == -2   ? p.tokens[row / c.group].split
+                                       : it.seq < 0 ? row / c.group + it.shift
+                                                    : row / c.group;
             if (tok < 0 || tok >= total) return bad("item token", k);
             const int packed = tok * c.group + row % c.group;
             if (it.seq >= 0 && seq[tok] != it.seq) return bad("item sequence", k);
@@ -56,7 +58,7 @@ static int check(const BatchLimits &c, const std::vector<int> &start, const std:
                 const int at = it.state0 + r;
                 if (at >= p.state_rows || state.count(at)) return bad("state rows meet", k);
                 state[at] = packed;
-                of_row[packed].push_back(at);
+                if (it.seq < 0 || last >= it.o0) of_row[packed].push_back(at);
             }
         }
     }
@@ -74,6 +76,8 @@ static int check(const BatchLimits &c, const std::vector<int> &start, const std:
             std::vector<int> want;
             for (int n = 0; n < p.head.prefix_chunks; n++) want.push_back(m.prefix_state + n * p.head.prefix_stride + h);
             for (int n = 0; n < m.own_chunks; n++) want.push_back(m.own_state + n * m.own_stride + h);
+            // a block's later rows may see a range of keys that this one does not: such a
+            // state holds no keys and is left out
             std::vector<int> &have = of_row[m.merge * c.group + h];
             std::sort(want.begin(), want.end());
             std::sort(have.begin(), have.end());
@@ -81,7 +85,9 @@ static int check(const BatchLimits &c, const std::vector<int> &start, const std:
             joined += have.size();
         }
     }
-    if (joined != state.size()) return bad("states that nothing joins", k);
+    size_t rows_joined = 0;
+    for (const auto &x : of_row) rows_joined += x.second.size();
+    if (joined != rows_joined) return bad("states that nothing joins", k);
     return 0;
 }
 
@@ -96,7 +102,7 @@ int main() {
         c.sequences = pick(1, 12);
         c.capacity = pick(1, 300);
         c.prefix_capacity = k % 3 ? pick(0, 900) : 0;
-        c.workgroups = k % 4 == 0 ? 16 : k % 4 == 1 ? 256 : k % 4 == 2 ? 1 : 768;
+        c.cus = k % 4 == 0 ? 16 : k % 4 == 1 ? 256 : k % 4 == 2 ? 1 : 64;
         const bool single = k % 5 == 0;
         std::vector<int> start(c.sequences), t(c.sequences);
         int total = 0;
@@ -109,6 +115,13 @@ int main() {
         const int prefix = c.prefix_capacity ? pick(0, c.prefix_capacity) : 0;
         if (check(c, start, t, prefix, k)) return 1;
         const BatchPlan p = batch_plan(c, start.data(), t.data(), prefix);
+        // graphs of this plan's t replay under plans for other positions
+        for (int j = 0; j < 4; j++) {
+            std::vector<int> other(c.sequences);
+            for (int s = 0; s < c.sequences; s++) other[s] = j == 0 ? c.capacity - t[s] : pick(0, c.capacity - t[s]);
+            const BatchPlan q = batch_plan(c, other.data(), t.data(), j == 1 ? 0 : c.prefix_capacity);
+            if (q.head.items > p.head.most_items) return bad("more items than a captured call launches", k);
+        }
         for (const BatchItem &it : p.items) (it.state0 < 0 ? wholes : splits)++;
     }
     if (!wholes || !splits) return bad("both kinds of items", -1);

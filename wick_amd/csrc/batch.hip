@@ -1,11 +1,14 @@
 // batch.hip -- attention of a batch's packed tokens over a shared prefix and the
 // sequences' own positions, and the cache writes that go with it.
 //
-// A workgroup (BatchItem) has 32 rows of one kv head -- a row is one (token, query head)
-// pair -- and walks its keys in steps of 128, each of its 4 waves 32 keys of a step.  Per
-// 32 keys a wave computes
-//   S^T [32 keys x 32 rows] = K Q^T,   P^T = exp2(S^T - m),   O^T [D x 32 rows] += V^T P^T
-// with v_mfma_f32_32x32x16_bf16.  Its four waves' states (m, l, O) are joined through LDS.
+// A workgroup (BatchItem) has some rows of one kv head -- a row is one (token, query head)
+// pair -- and walks its keys.  Per 32 keys a wave computes
+//   S^T [keys x rows] = K Q^T,   P^T = exp2(S^T - m),   O^T [D x rows] += V^T P^T
+// with the running maximum m and sum l of each row.  Items of up to 128 rows are wide: each of
+// the 4 waves has 32 rows, all of them the same keys, whose operands they prepare together in
+// LDS (v_mfma_f32_32x32x16_bf16).  Items of up to 16 rows are narrow: the waves have the same rows
+// and every fourth 32 keys each, and join their states through LDS at the end
+// (v_mfma_f32_16x16x32_bf16).
 //
 // f32 products on the bf16 matrix cores.  x = x1 + x2 + x3, each part the bf16 nearest to
 // what the ones before it leave (8 + 8 + 8 significant bits: exact but for the last part's
@@ -26,6 +29,8 @@
 // D / 32 instructions, so that a lane reads D / 32 adjacent values of a key, and a half
 // wave a whole key.
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "batch_kernels.h"
 #include "wave_ops.h"
@@ -132,37 +137,166 @@ __device__ __forceinline__ Parts<1> parts8(const __bf16 *x) {
     return r;
 }
 
+// The parts of 2 values, to places j and j + 1.
+__device__ __forceinline__ void split2(const float *x, Parts<3> &r, int j) {
+    f32x2 v = {x[0], x[1]};
+#pragma unroll
+    for (int p = 0; p < 3; p++) {
+        const b16x2 h = __builtin_convertvector(v, b16x2);
+        r.part[p][j] = h[0];
+        r.part[p][j + 1] = h[1];
+        v -= __builtin_convertvector(h, f32x2);
+    }
+}
+__device__ __forceinline__ void split2(const __bf16 *x, Parts<1> &r, int j) {
+    r.part[0][j] = x[0];
+    r.part[0][j + 1] = x[1];
+}
+
+// The parts of 4 values.
+__device__ __forceinline__ void parts4(const float *x, b16x4 (&part)[3]) {
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+        f32x2 v = {x[i], x[i + 1]};
+#pragma unroll
+        for (int p = 0; p < 3; p++) {
+            const b16x2 h = __builtin_convertvector(v, b16x2);
+            part[p][i] = h[0];
+            part[p][i + 1] = h[1];
+            v -= __builtin_convertvector(h, f32x2);
+        }
+    }
+}
+__device__ __forceinline__ void parts4(const __bf16 *x, b16x4 (&part)[1]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) part[0][i] = x[i];
+}
+
 __device__ __forceinline__ float other_half(float v) {
     const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float((threadIdx.x & 32) ? p[0] : p[1]);
 }
 
+// What the kernel's shape fixes.
+template <int D, class T>
+struct Shape {
+    static constexpr int KS = D / 16;                // QK instructions per product of parts and 32 keys
+    static constexpr int NB = D >= 32 ? D / 32 : 1;  // 32-dimension blocks of O
+    static constexpr int KP = sizeof(T) == 4 ? 3 : 1;
+    // a wide item's tile: 64 keys, or 32 where the parts of 64 would not leave room for two
+    // workgroups on a CU
+    static constexpr int KT = D == 128 && KP == 3 ? 32 : 64;
+    // q's third parts lie in LDS where all of them would not leave the registers for two
+    static constexpr int QP = D == 128 ? 2 : 3;
+    static constexpr int KF = KT / 32 * KS, VF = KT / 16 * NB;  // operands of a tile: K's, V's
+    // a narrow item's, with 16x16x32 instructions
+    static constexpr int KS16 = D >= 32 ? D / 32 : 1, NB16 = D / 16;
+};
+
+// Operands lie as the instruction takes them: a wave reads one with its lanes side by side.
+template <int D, class T>
+struct Tile {
+    using S = Shape<D, T>;
+    b16x8 k[S::KP][S::KF][64], v[S::KP][S::VF][64];
+};
+template <int KP, int N>
+__device__ __forceinline__ Parts<KP> read(const b16x8 (&x)[KP][N][64], int i, int lane) {
+    Parts<KP> r;
+#pragma unroll
+    for (int p = 0; p < KP; p++) r.part[p] = x[p][i][lane];
+    return r;
+}
+
+// The four waves' states of a narrow item, by row.
 template <int D>
-struct Lds {
-    float o[4][32][D + 4];  // the waves' O, by row
-    float m[4][32], l[4][32];
-    int redo[32];
+struct Join {
+    float o[4][kBatchRows][D + 4];
+    float m[4][kBatchRows], l[4][kBatchRows];
+    int redo[kBatchRows];
+};
+
+// A tile's keys or values on their way to LDS: each wave has every fourth K operand, and
+// of V's 16-key groups every fourth half.  Keys past `end` are the last one again.
+template <int D, class T>
+struct StageK {
+    using S = Shape<D, T>;
+    static constexpr int N = (S::KF + 3) / 4;
+    T x[N][8];
+
+    // k: the tile's first key, of n left
+    __device__ __forceinline__ void load(const T *k, int n, int wave, int col, int half) {
+        if (S::KF < 4 && wave >= S::KF) return;
+        // operand wave + 4 u: 32 keys, 16 dimensions
+        const int sub = S::KS >= 4 ? 0 : wave / S::KS, ks = S::KS >= 4 ? wave : wave % S::KS;
+#pragma unroll
+        for (int u = 0; u < N; u++)
+            load_n<8>(k + 16 * (ks + 4 * u % S::KS) + (unsigned)(min(32 * (sub + 4 * u / S::KS) + col, n - 1) * D + 8 * half),
+                      x[u]);
+    }
+    // The split into parts and the write in UNITS steps, each two values of a lane's 8.
+    static constexpr int UNITS = 4 * N;
+    Parts<S::KP> y;
+    __device__ __forceinline__ static b16x8 *place(Tile<D, T> &t, int wave, int lane) { return &t.k[0][wave][lane]; }
+    __device__ __forceinline__ void store(int i, b16x8 *at, int wave) {
+        const int u = i / 4, j = 2 * (i % 4);
+        if (S::KF < 4 && wave >= S::KF) return;
+        split2(x[u] + j, y, j);
+        if (j == 6)
+#pragma unroll
+            for (int p = 0; p < S::KP; p++) at[(p * S::KF + 4 * u) * 64] = y.part[p];
+    }
+};
+template <int D, class T>
+struct StageV {
+    using S = Shape<D, T>;
+    static constexpr int N = S::KT / 32;
+    T x[N][4][S::NB];
+
+    __device__ __forceinline__ void load(const T *v, int n, int wave, int col, int half) {
+#pragma unroll
+        for (int u = 0; u < N; u++) {
+            const int h = wave + 4 * u;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                load_n<S::NB>(v + (unsigned)(min(8 * h + 4 * half + j, n - 1) * D + (D < 32 ? col % D : S::NB * col)), x[u][j]);
+        }
+    }
+    // The same in UNITS steps of a dimension.
+    static constexpr int UNITS = N * S::NB;
+    __device__ __forceinline__ static b16x4 *place(Tile<D, T> &t, int wave, int lane) {
+        return reinterpret_cast<b16x4 *>(&t.v[0][wave / 2 * S::NB][lane]) + wave % 2;
+    }
+    __device__ __forceinline__ void store(int i, b16x4 *at) const {
+        const int u = i / S::NB, b = i % S::NB;
+        T y[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) y[j] = x[u][j][b];
+        b16x4 part[S::KP];
+        parts4(y, part);
+#pragma unroll
+        for (int p = 0; p < S::KP; p++) at[(p * S::VF + 2 * u * S::NB + b) * 128] = part[p];
+    }
 };
 
 // One row again in f32, key by key by one wave, over the item's keys that it sees: the
 // definition itself, for rows with a value that the parts have no room for.  Lane d has
-// the dimensions d, d + 64; o gets them unscaled.
+// the dimensions d, d + 64.
 template <int D, class T>
-__device__ void redo_row(const BatchArgs &a, const BatchItem &it, const float *q, const T *pk, const T *pv, const T *k,
-                         const T *v, int own_end, float *m_out, float *l_out, float *o_out) {
+__device__ __noinline__ void redo_row(const float *q, float scale, const T *pk, const T *pv, int p0, int p1, const T *k,
+                                      const T *v, int o0, int o1, bool direct, float *dst, float *m_out, float *l_out) {
     const int lane = threadIdx.x & 63;
     constexpr int N = (D + 63) / 64;
     float x[N], acc[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        x[i] = lane + 64 * i < D ? q[lane + 64 * i] * a.scale : 0.0f;
+        x[i] = lane + 64 * i < D ? q[lane + 64 * i] * scale : 0.0f;
         acc[i] = 0.0f;
     }
     float m = kNoMax, l = 0.0f;
     for (int part = 0; part < 2; part++) {
         const T *kk = part ? k : pk, *vv = part ? v : pv;
-        const int end = part ? own_end : it.p1;
-        for (int key = part ? it.o0 : it.p0; key < end; key++) {
+        const int end = part ? o1 : p1;
+        for (int key = part ? o0 : p0; key < end; key++) {
             float s = 0.0f;
 #pragma unroll
             for (int i = 0; i < N; i++)
@@ -182,248 +316,535 @@ __device__ void redo_row(const BatchArgs &a, const BatchItem &it, const float *q
                 if (lane + 64 * i < D) acc[i] += p * (float)vv[(size_t)key * D + lane + 64 * i];
         }
     }
-    *m_out = m;
-    *l_out = l;
 #pragma unroll
     for (int i = 0; i < N; i++)
-        if (lane + 64 * i < D) o_out[lane + 64 * i] = acc[i];
+        if (lane + 64 * i < D) dst[lane + 64 * i] = direct ? acc[i] / l : acc[i];
+    if (!direct && lane == 0) {
+        *m_out = m;
+        *l_out = l;
+    }
 }
 
+// The softmax state of a wave's 32 rows (row lane % 32), and what a tile of 32 keys does to it.
 template <int D, class T>
-__global__ __launch_bounds__(256) void batch_attend_kernel(BatchArgs a) {
-    constexpr int KS = D / 16;               // QK instructions per part product
-    constexpr int NB = D >= 32 ? D / 32 : 1;  // 32-dimension blocks of O
-    constexpr int KP = sizeof(T) == 4 ? 3 : 1;
-    __shared__ Lds<D> lds;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, col = lane & 31, half = lane >> 5;
+struct Rows {
+    using S = Shape<D, T>;
+    Parts<S::QP> q[S::KS];
+    b16x8 *rest;  // q's third parts where they are not in registers
+    f32x16 o[S::NB];
+    float m, l;  // l: of the keys in this lane
+
+    __device__ __forceinline__ void begin(const float *src, float scale, int half, b16x8 *third) {
+        rest = third;
+#pragma unroll
+        for (int ks = 0; ks < S::KS; ks++) {
+            float x[8];
+            load_n<8>(src + 16 * ks + 8 * half, x);
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] *= scale;
+            const Parts<3> y = split8(x);
+#pragma unroll
+            for (int p = 0; p < S::QP; p++) q[ks].part[p] = y.part[p];
+            if constexpr (S::QP < 3) rest[64 * ks] = y.part[2];
+        }
+#pragma unroll
+        for (int b = 0; b < S::NB; b++) o[b] = f32x16{};
+        m = kNoMax;
+        l = 0.0f;
+    }
+
+    __device__ __forceinline__ Parts<3> query(int ks) const {
+        Parts<3> r;
+#pragma unroll
+        for (int p = 0; p < S::QP; p++) r.part[p] = q[ks].part[p];
+        if constexpr (S::QP < 3) r.part[2] = rest[64 * ks];
+        return r;
+    }
+
+    // scores s of the keys key0..: keys past `last` are hidden, the reference maximum follows
+    template <bool MASK>
+    __device__ __forceinline__ void scores(f32x16 &s, int key0, int half, int last) {
+        if constexpr (MASK) {
+            const int left = last - key0 - 4 * half;
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[i] = i % 4 + 8 * (i / 4) > left ? -INFINITY : s[i];
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
+        top = fmaxf(top, other_half(top));
+        if (__any(top > m + kSlack)) {
+            const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < S::NB; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[b][i] *= f;
+            m = to;
+        }
+    }
+
+    // the weights of scores s[8 kk + j], s[8 kk + j + 1] and their parts
+    __device__ __forceinline__ void weight2(f32x16 &s, Parts<3> &w, int kk, int j) {
+        float p[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            p[i] = __builtin_amdgcn_exp2f(s[8 * kk + j + i] - m);
+            l += p[i];
+        }
+        split2(p, w, j);
+    }
+};
+
+__device__ __forceinline__ f32x4 mfma16(b16x8 a, b16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 product(const Parts<3> &a, const Parts<3> &b, f32x4 c) {
+    c = mfma16(a.part[2], b.part[0], c);
+    c = mfma16(a.part[0], b.part[2], c);
+    c = mfma16(a.part[1], b.part[1], c);
+    c = mfma16(a.part[1], b.part[0], c);
+    c = mfma16(a.part[0], b.part[1], c);
+    return mfma16(a.part[0], b.part[0], c);
+}
+__device__ __forceinline__ f32x4 product(const Parts<1> &a, const Parts<3> &b, f32x4 c) {
+    c = mfma16(a.part[0], b.part[2], c);
+    c = mfma16(a.part[0], b.part[1], c);
+    return mfma16(a.part[0], b.part[0], c);
+}
+
+// Up to 16 rows (row lane % 16) against 32 keys at a time, the operands straight from
+// memory.  The 16x16x32 instruction gives lane l row or column l % 16 and the contracted indices
+// 8 (l / 16)..; scores leave it with keys 4 (l / 16) + i of each 16, so V's operand takes
+// keys 4 (l / 16) + j and, for j >= 4, 16 + 4 (l / 16) + j - 4.
+template <int D, class T>
+struct Few {
+    using S = Shape<D, T>;
+    static constexpr int KS = S::KS16, NB = S::NB16;
+    Parts<3> q[KS];
+    f32x4 o[NB];
+    float m, l;
+    T k[2][KS][8], v[8][NB];
+
+    __device__ __forceinline__ void begin(const float *src, float scale, int quad) {
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            float x[8] = {};
+            if (D >= 32 || quad < 2) load_n<8>(src + 32 * ks + 8 * quad, x);
+#pragma unroll
+            for (int j = 0; j < 8; j++) x[j] *= scale;
+            q[ks] = split8(x);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) o[b] = f32x4{};
+        m = kNoMax;
+        l = 0.0f;
+    }
+
+    // of n keys left at p
+    __device__ __forceinline__ void load_k(const T *p, int n, int col, int quad) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const unsigned at = min(16 * u + col, n - 1) * D + 8 * (D >= 32 ? quad : quad & 1);
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) load_n<8>(p + 32 * ks + at, k[u][ks]);
+        }
+    }
+    __device__ __forceinline__ void load_v(const T *p, int n, int col, int quad) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            load_n<NB>(p + (unsigned)(min(16 * (j / 4) + 4 * quad + j % 4, n - 1) * D + NB * col), v[j]);
+    }
+
+    __device__ __forceinline__ void scores(f32x4 (&s)[2]) const {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            s[u] = f32x4{};
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) s[u] = product(parts8(k[u][ks]), q[ks], s[u]);  // 16 dimensions: q's rest is 0
+        }
+    }
+
+    // keys past `left` of the 32 are hidden
+    __device__ __forceinline__ void values(f32x4 (&s)[2], bool mask, int left) {
+        if (mask) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[i / 4][i % 4] = 16 * (i / 4) + i % 4 > left ? -INFINITY : s[i / 4][i % 4];
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) top = fmaxf(top, s[i / 4][i % 4]);
+        top = rows_max(top);
+        if (__any(top > m + kSlack)) {
+            const float to = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - to);
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < NB; b++) o[b] *= f;
+            m = to;
+        }
+        float p[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            p[i] = __builtin_amdgcn_exp2f(s[i / 4][i % 4] - m);
+            l += p[i];
+        }
+        const Parts<3> w = split8(p);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            T y[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = v[j][b];
+            o[b] = product(parts8(y), w, o[b]);
+        }
+    }
+};
+
+template <int D, class T>
+__global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
+    using S = Shape<D, T>;
+    constexpr int KS = S::KS, NB = S::NB, KT = S::KT;
+    __shared__ union {
+        Join<D> join;
+        struct {
+            Tile<D, T> tile;
+            b16x8 third[S::QP < 3 ? 4 : 1][S::QP < 3 ? KS : 1][64];
+        };
+    } lds;
+    const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // the same in all lanes
     const int heads = a.group * a.kv_heads;
 
-    // the plan in memory is another one than at the call (a replayed graph)
-    if (a.head->shape != a.shape) {
+    // the plan in memory does not fit the call (a replayed graph)
+    const int work = a.head->items * a.kv_heads;
+    if (a.head->shape != a.shape || work > (int)gridDim.x) {
         const size_t n = (size_t)a.total * heads * D;
         for (size_t i = (size_t)blockIdx.x * 256 + tid; i < n; i += (size_t)gridDim.x * 256)
             a.att[i] = __builtin_nanf("");
         return;
     }
-    const int work = a.head->items * a.kv_heads;
-    for (int w = blockIdx.x; w < work; w += gridDim.x) {
-        const BatchItem it = a.items[w / a.kv_heads];
-        const int kh = w % a.kv_heads;
+    if ((int)blockIdx.x >= work) return;
+    {
+        const BatchItem it = a.items[blockIdx.x / a.kv_heads];
+        const int kh = blockIdx.x % a.kv_heads;
         const T *pk = static_cast<const T *>(a.pk) + (size_t)kh * a.prefix_capacity * D;
         const T *pv = static_cast<const T *>(a.pv) + (size_t)kh * a.prefix_capacity * D;
         const size_t own = it.seq < 0 ? 0 : ((size_t)it.seq * a.kv_heads + kh) * a.capacity * D;
         const T *ok = static_cast<const T *>(a.k) + own, *ov = static_cast<const T *>(a.v) + own;
+        const bool direct = it.state0 < 0;
 
-        // a row's token and place in q and att
+        // row r of the item: its place in q and att, its last own key, its states
         auto row_at = [&](int r) {
             const int row = it.row0 + r, t = row / a.group, h = row - t * a.group;
-            const int token = it.seq < 0 ? a.tokens[t].split : t;
+            const int token = it.seq >= 0 ? t : it.seq == -1 ? t + it.shift : a.tokens[t].split;
             return ((size_t)token * heads + kh * a.group + h) * D;
         };
-        const int r = min(col, it.nrows - 1);
-        const int last = it.seq < 0 ? -1 : (it.row0 + r) / a.group + it.shift;  // the row's last own key
-        const int first_last = it.seq < 0 ? -1 : it.row0 / a.group + it.shift;  // the first row's
+        auto last_of = [&](int r) { return it.seq < 0 ? -1 : (it.row0 + r) / a.group + it.shift; };
+        auto state_at = [&](int r) { return (size_t)kh * a.state_rows + it.state0 + r; };
+        auto redo = [&](int r) {
+            const size_t at = direct ? 0 : state_at(r);
+            redo_row<D, T>(a.q + row_at(r), a.scale, pk, pv, it.p0, it.p1, ok, ov, it.o0, min(it.o1, last_of(r) + 1), direct,
+                           direct ? a.att + row_at(r) : a.po + at * D, a.pm + at, a.pl + at);
+        };
 
-        Parts<3> q[KS];
-        {
-            const float *src = a.q + row_at(r);
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++) {
-                float x[8];
-                load_n<8>(src + 16 * ks + 8 * half, x);
-#pragma unroll
-                for (int j = 0; j < 8; j++) x[j] *= a.scale;
-                q[ks] = split8(x);
-            }
-        }
-        f32x16 o[NB];
-#pragma unroll
-        for (int b = 0; b < NB; b++) o[b] = f32x16{};
-        float m = kNoMax, l = 0.0f;
+        if (it.nrows > kBatchRows) {
+            // this wave's rows
+            const int r0 = 32 * wave, nr = min(32, it.nrows - r0);
+            const int r = max(0, min(r0 + col, it.nrows - 1));
+            const int last = last_of(r), first_last = last_of(min(r0, it.nrows - 1)),
+                      end_last = last_of(min(r0 + 32, it.nrows) - 1);
+            Rows<D, T> st;
 
-        for (int part = 0; part < 2; part++) {
-            const T *kk = part ? ok : pk, *vv = part ? ov : pv;
-            const int begin = part ? it.o0 : it.p0, end = part ? it.o1 : it.p1;
-            for (int key0 = begin + 32 * wave; key0 < end; key0 += kBatchStep) {
-                f32x16 s{};
-                const T *krow = kk + (size_t)min(key0 + col, end - 1) * D + 8 * half;
+            // The tiles of the prefix, then those of the own keys.  While the scores of a tile
+            // are summed, its values are split into parts and written to LDS; while its values
+            // are, the next tile's keys.
+            StageK<D, T> sk;
+            StageV<D, T> sv;
+            const int tp = (it.p1 - it.p0 + KT - 1) / KT, tiles = tp + (it.o1 - it.o0 + KT - 1) / KT;
+            auto first_key = [&](int t) { return t >= tp ? it.o0 + (t - tp) * KT : it.p0 + t * KT; };
+            auto load_k = [&](int t) {
+                const bool o = t >= tp;
+                const int key = first_key(t);
+                sk.load((o ? ok : pk) + (size_t)key * D, (o ? it.o1 : it.p1) - key, wave, col, half);
+            };
+            auto load_v = [&](int t) {
+                const bool o = t >= tp;
+                const int key = first_key(t);
+                sv.load((o ? ov : pv) + (size_t)key * D, (o ? it.o1 : it.p1) - key, wave, col, half);
+            };
+            b16x8 *const kat = sk.place(lds.tile, wave, lane);
+            b16x4 *const vat = sv.place(lds.tile, wave, lane);
+            load_k(0);
+            load_v(0);
+            st.begin(a.q + row_at(r), a.scale, half, &lds.third[S::QP < 3 ? wave : 0][0][lane]);
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) {
-                    T x[8];
-                    load_n<8>(krow + 16 * ks, x);
-                    s = product(parts8(x), q[ks], s);
-                }
-                if (key0 + 32 > end || (part && key0 + 31 > first_last)) {
+            for (int i = 0; i < sk.UNITS; i++) sk.store(i, kat, wave);
+            load_k(min(1, tiles - 1));  // past the last tile the last one again: no one reads it
+            __syncthreads();
+            // a tile for this wave; MASK: some of its keys are past the end or hidden from some rows
+            auto tile = [&](auto mask, int t, int tile0, int seen) {
+                constexpr bool MASK = decltype(mask)::value;
+                f32x16 s[KT / 32];
+                {
+                    // one group: an operand's products, the next operand's read, a share of the split
+                    constexpr int G = S::KF;
+                    Parts<S::KP> x = read(lds.tile.k, 0, lane), y;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int key = key0 + 4 * half + i % 4 + 8 * (i / 4);
-                        if (key >= end || (part && key > last)) s[i] = -INFINITY;
+                    for (int g = 0; g < G; g++) {
+                        if (g + 1 < G) y = read(lds.tile.k, g + 1, lane);
+                        if (g % KS == 0) s[g / KS] = f32x16{};
+                        s[g / KS] = product(x, st.query(g % KS), s[g / KS]);
+#pragma unroll
+                        for (int i = g * sv.UNITS / G; i < (g + 1) * sv.UNITS / G; i++) sv.store(i, vat);
+                        x = y;
                     }
                 }
-                float top = s[0];
+                load_v(min(t + 1, tiles - 1));
+                __syncthreads();
+                constexpr int G = 2 * NB, UNITS = sk.UNITS * 32 / KT;  // of a 32-key part
 #pragma unroll
-                for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
-                top = fmaxf(top, other_half(top));
-                if (__any(top > m + kSlack)) {
-                    const float to = fmaxf(m, top), f = exp2f(m - to);
-                    l *= f;
+                for (int sub = 0; sub < KT / 32; sub++) {
+                    Parts<S::KP> x = read(lds.tile.v, sub * G, lane), y;
+                    st.template scores<MASK>(s[sub], tile0 + 32 * sub, half, seen);
+                    Parts<3> w8[2];
 #pragma unroll
-                    for (int b = 0; b < NB; b++)
+                    for (int j = 0; j < 8; j += 2) st.weight2(s[sub], w8[0], 0, j);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) o[b][i] *= f;
-                    m = to;
-                }
+                    for (int g = 0; g < G; g++) {
+                        if (g + 1 < G) y = read(lds.tile.v, sub * G + g + 1, lane);
+                        st.o[g % NB] = product(x, w8[g / NB], st.o[g % NB]);
+                        if (g < NB)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    s[i] = __builtin_amdgcn_exp2f(s[i] - m);
-                    l += s[i];
-                }
+                            for (int j = g * 4 / NB; j < (g + 1) * 4 / NB; j++) st.weight2(s[sub], w8[1], 1, 2 * j);
 #pragma unroll
-                for (int kk2 = 0; kk2 < 2; kk2++) {
-                    float p[8];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) p[j] = s[8 * kk2 + j];
-                    const Parts<3> pp = split8(p);
-                    T x[8][NB];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const int key = min(key0 + 16 * kk2 + (j / 4) * 8 + 4 * half + j % 4, end - 1);
-                        load_n<NB>(vv + (size_t)key * D + (D < 32 ? col % D : NB * col), x[j]);
-                    }
-#pragma unroll
-                    for (int b = 0; b < NB; b++) {
-                        T y[8];
-#pragma unroll
-                        for (int j = 0; j < 8; j++) y[j] = x[j][b];
-                        o[b] = product(parts8(y), pp, o[b]);
-                    }
-                }
-            }
-        }
-        l += other_half(l);
+                        for (int i = g * UNITS / G; i < (g + 1) * UNITS / G; i++) sk.store(sub * UNITS + i, kat, wave);
 
-        // join the waves' states: O by row through LDS
-        if (half == 0) {
-            lds.m[wave][col] = m;
-            lds.l[wave][col] = l;
-        }
-        if (tid < 32) lds.redo[tid] = 0;
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int d = 4 * half + i % 4 + 8 * (i / 4);
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-                if (NB * d + b < D) lds.o[wave][col][NB * d + b] = o[b][i];
-        }
-        __syncthreads();
-        {
-            // 8 threads a row, D / 8 dimensions each
-            constexpr int E = D / 8;
-            const int row = tid >> 3, d0 = (tid & 7) * E;
-            float to = lds.m[0][row];
-#pragma unroll
-            for (int i = 1; i < 4; i++) to = fmaxf(to, lds.m[i][row]);
-            float sum = 0.0f, acc[E];
-#pragma unroll
-            for (int e = 0; e < E; e++) acc[e] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float f = exp2f(lds.m[i][row] - to);
-                sum += f * lds.l[i][row];
-#pragma unroll
-                for (int e = 0; e < E; e++) acc[e] += f * lds.o[i][row][d0 + e];
+                        x = y;
+                    }
+                }
+                load_k(min(t + 2, tiles - 1));
+                __syncthreads();
+            };
+            // One loop after the other, so that O stays where it is: of the prefix and then of the
+            // own keys the tiles that all rows of the wave see whole, those that they see in
+            // part, and last the tiles that the other waves still need.
+            int t = 0;
+            for (int part = 0; part < 2; part++) {
+                const int begin = part ? it.o0 : it.p0, end = part ? it.o1 : it.p1;
+                // keys that every row sees, and that any row does
+                const int all = max(0, (part ? min(end, first_last + 1) : end) - begin);
+                const int any = max(0, (part ? min(end, end_last + 1) : end) - begin);
+                if (nr <= 0) break;
+                const int t0 = t;
+                for (const int stop = t0 + all / KT; t < stop; t++) tile(std::false_type{}, t, 0, 0);
+                for (const int stop = t0 + (any + KT - 1) / KT; t < stop; t++)
+                    tile(std::true_type{}, t, begin + (t - t0) * KT, part ? min(last, end - 1) : end - 1);
             }
+            for (; t < tiles; t++) {
+#pragma unroll
+                for (int i = 0; i < sv.UNITS; i++) sv.store(i, vat);
+                load_v(min(t + 1, tiles - 1));
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < sk.UNITS; i++) sk.store(i, kat, wave);
+                load_k(min(t + 2, tiles - 1));
+                __syncthreads();
+            }
+            const float sum = st.l + other_half(st.l);
             bool odd = !(fabsf(sum) < INFINITY);
 #pragma unroll
-            for (int e = 0; e < E; e++) odd |= !(fabsf(acc[e]) < INFINITY);
-            if (odd && row < it.nrows) lds.redo[row] = 1;
-            __syncthreads();
-            // each thread has read its own values of all waves and nobody else's
+            for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int e = 0; e < E; e++) lds.o[0][row][d0 + e] = acc[e];
-            if ((tid & 7) == 0) {
-                lds.m[0][row] = to;
-                lds.l[0][row] = sum;
-            }
-        }
-        __syncthreads();
-        for (int rr = wave; rr < it.nrows; rr += 4)
-            if (lds.redo[rr]) {
-                float rm, rl;
-                const int seen = it.seq < 0 ? 0 : min(it.o1, (it.row0 + rr) / a.group + it.shift + 1);
-                redo_row<D, T>(a, it, a.q + row_at(rr), pk, pv, ok, ov, seen, &rm, &rl, lds.o[0][rr]);
-                lds.m[0][rr] = rm;
-                lds.l[0][rr] = rl;
-            }
-        __syncthreads();
-        {
-            constexpr int E = D / 8;
-            const int row = tid >> 3, d0 = (tid & 7) * E;
-            if (row < it.nrows) {
-                const float sum = lds.l[0][row], f = it.state0 < 0 ? 1.0f / sum : 1.0f;
-                float *dst;
-                if (it.state0 < 0) {
-                    dst = a.att + row_at(row) + d0;
-                } else {
-                    const size_t at = (size_t)kh * a.state_rows + it.state0 + row;
-                    dst = a.po + at * D + d0;
-                    if (d0 == 0) {
-                        a.pm[at] = lds.m[0][row];
-                        a.pl[at] = sum;
+                for (int i = 0; i < 16; i++) odd |= !(fabsf(st.o[b][i]) < INFINITY);
+            const unsigned long long odds = __ballot(odd && col < nr);
+            const unsigned again = (unsigned)odds | (unsigned)(odds >> 32);
+            if (col < nr && !(again >> col & 1)) {
+                const float f = direct ? 1.0f / sum : 1.0f;
+                float *dst = direct ? a.att + row_at(r) : a.po + state_at(r) * D;
+#pragma unroll
+                for (int g = 0; g < 4; g++) {
+                    float x[4 * NB];  // dimensions NB (4 half + 8 g)...
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int b = 0; b < NB; b++) x[NB * i + b] = st.o[b][4 * g + i] * f;
+                    if (NB * (4 * half + 8 * g) < D) {
+#pragma unroll
+                        for (int i = 0; i < 4 * NB; i += 4)
+                            *reinterpret_cast<f32x4 *>(dst + NB * (4 * half + 8 * g) + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
                     }
                 }
-#pragma unroll
-                for (int e = 0; e < E; e++) dst[e] = lds.o[0][row][d0 + e] * f;
+                if (!direct && half == 0) {
+                    a.pm[state_at(r)] = st.m;
+                    a.pl[state_at(r)] = sum;
+                }
             }
+            for (int i = 0; i < 32; i++)
+                if (again >> i & 1) redo(r0 + i);
+            return;
         }
+
+        {
+            const int c = lane & 15, quad = lane >> 4, r = min(c, it.nrows - 1);
+            const int last = last_of(r), first_last = last_of(0);
+            // this wave's tiles: every fourth 32 keys of the prefix, then of the own keys
+            const int np = max(0, (it.p1 - it.p0 - 32 * wave + 127) / 128);
+            const int tiles = np + max(0, (it.o1 - it.o0 - 32 * wave + 127) / 128);
+            auto first_key = [&](int t) { return 32 * wave + (t < np ? it.p0 + 128 * t : it.o0 + 128 * (t - np)); };
+            Few<D, T> st;
+            auto load_k = [&](int t) {
+                const int key = first_key(t);
+                st.load_k((t < np ? pk : ok) + (size_t)key * D, (t < np ? it.p1 : it.o1) - key, c, quad);
+            };
+            if (tiles > 0) load_k(0);
+            st.begin(a.q + row_at(r), a.scale, quad);
+            for (int t = 0; t < tiles; t++) {
+                const bool o = t >= np;
+                const int key0 = first_key(t), end = o ? it.o1 : it.p1;
+                st.load_v((o ? ov : pv) + (size_t)key0 * D, end - key0, c, quad);
+                f32x4 s[2];
+                st.scores(s);
+                load_k(min(t + 1, tiles - 1));  // past the last tile the last one again
+                st.values(s, key0 + 32 > end || (o && key0 + 31 > first_last),
+                          (o ? min(last, end - 1) : end - 1) - key0 - 4 * quad);
+            }
+            const float l = rows_sum(st.l);
+            // join the waves' states: O by row through LDS
+            Join<D> &j = lds.join;
+            if (quad == 0) {
+                j.m[wave][c] = st.m;
+                j.l[wave][c] = l;
+            }
+            if (tid < kBatchRows) j.redo[tid] = 0;
+            constexpr int NB16 = S::NB16;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int b = 0; b < NB16; b++) j.o[wave][c][NB16 * (4 * quad + i) + b] = st.o[b][i];
+        }
+        Join<D> &j = lds.join;
         __syncthreads();
+        // 16 threads a row, D / 16 dimensions each
+        constexpr int E = D / 16;
+        const int row = tid >> 4, d0 = (tid & 15) * E;
+        float to = j.m[0][row];
+#pragma unroll
+        for (int i = 1; i < 4; i++) to = fmaxf(to, j.m[i][row]);
+        float sum = 0.0f, acc[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) acc[e] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float f = exp2f(j.m[i][row] - to);
+            sum += f * j.l[i][row];
+#pragma unroll
+            for (int e = 0; e < E; e++) acc[e] += f * j.o[i][row][d0 + e];
+        }
+        bool odd = !(fabsf(sum) < INFINITY);
+#pragma unroll
+        for (int e = 0; e < E; e++) odd |= !(fabsf(acc[e]) < INFINITY);
+        if (odd && row < it.nrows) j.redo[row] = 1;
+        __syncthreads();
+        if (row < it.nrows && !j.redo[row]) {
+            const float f = direct ? 1.0f / sum : 1.0f;
+            float *dst = direct ? a.att + row_at(row) + d0 : a.po + state_at(row) * D + d0;
+            if (!direct && d0 == 0) {
+                a.pm[state_at(row)] = to;
+                a.pl[state_at(row)] = sum;
+            }
+#pragma unroll
+            for (int e = 0; e < E; e++) dst[e] = acc[e] * f;
+        }
+        for (int i = wave; i < it.nrows; i += 4)
+            if (j.redo[i]) redo(i);
     }
 }
 
-// A wave joins one row's states: weights 2^(m_i - max), att = sum w O / sum w l.  Up to 64
-// states at a time have a lane each; for the sum of O, D / 4 lanes read one state.
-template <int D>
+// W waves join one row's states: with the largest m, weights 2^(m_i - m), att = sum w O /
+// sum w l.  D / 4 lanes read a state, 8 states in flight each; their running sums are
+// joined last, always in the same order.
+template <int D, int W>
 __global__ __launch_bounds__(256) void batch_merge_kernel(BatchArgs a) {
-    constexpr int L = D / 4, G = 64 / L;  // lanes of a state, states at once
-    const int lane = threadIdx.x & 63, g = lane / L, d = 4 * (lane % L);
+    constexpr int L = D / 4, G = 64 * W / L, B = 8;  // lanes of a state, states at once, and on their way
+    __shared__ float part[W > 1 ? W : 1][D + 2];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = 4 * (lane % L);
+    const int g = (W > 1 ? wave * (64 / L) : 0) + lane / L;
     const int heads = a.group * a.kv_heads;
     if (a.head->shape != a.shape) return;
-    const int work = a.head->merges * heads, prefix_chunks = a.head->prefix_chunks;
-    for (int w = blockIdx.x * 4 + (threadIdx.x >> 6); w < work; w += gridDim.x * 4) {
+    const int work = a.head->merges * heads, prefix_chunks = a.head->prefix_chunks, stride = a.head->prefix_stride;
+    constexpr int R = 4 / W;  // rows of a workgroup
+    for (int w = blockIdx.x * R + (W > 1 ? 0 : wave); w < work; w += gridDim.x * R) {
         const int i = w / heads, head = w - i * heads, kh = head / a.group, h = head - kh * a.group;
         const BatchToken t = a.tokens[i];
-        const size_t base = (size_t)kh * a.state_rows;
+        const size_t base = (size_t)kh * a.state_rows + h;
         const int n = prefix_chunks + t.own_chunks;
-        auto state = [&](int c) {
-            const int row = c < prefix_chunks ? t.prefix_state + c * a.head->prefix_stride
-                                              : t.own_state + (c - prefix_chunks) * t.own_stride;
-            return base + row + h;
-        };
-        float top = kNoMax;
-        for (int c = lane; c < n; c += 64) top = fmaxf(top, a.pm[state(c)]);
-        top = wave_max(top);
-        float sum = 0.0f;
+        float m = kNoMax, l = 0.0f;
         f32x4 acc{};
-        for (int c0 = 0; c0 < n; c0 += 64) {
-            float f = 0.0f;
-            if (c0 + lane < n) {
-                const size_t at = state(c0 + lane);
-                f = exp2f(a.pm[at] - top);
-                sum += f * a.pl[at];
-            }
-            const int m = min(64, n - c0);
-            for (int c = 0; c < m; c += G) {
-                const float fc = __shfl(f, min(c + g, 63), 64);
-                if (c + g < m) acc += fc * *reinterpret_cast<const f32x4 *>(a.po + state(c0 + c + g) * D + d);
-            }
-        }
-        sum = wave_sum(sum);
+        for (int c0 = g; c0 < n; c0 += B * G) {
+            f32x4 o[B];
+            float mm[B], ll[B], top = m;
 #pragma unroll
-        for (int x = L; x < 64; x <<= 1)
+            for (int b = 0; b < B; b++) {
+                const int c = min(c0 + b * G, n - 1);
+                const size_t at = base + (c < prefix_chunks ? t.prefix_state + (size_t)c * stride
+                                                            : t.own_state + (size_t)(c - prefix_chunks) * t.own_stride);
+                o[b] = *reinterpret_cast<const f32x4 *>(a.po + at * D + d);
+                mm[b] = a.pm[at];
+                ll[b] = a.pl[at];
+            }
+#pragma unroll
+            for (int b = 0; b < B; b++) top = fmaxf(top, mm[b]);
+            const float old = exp2f(m - top);
+            l *= old;
+            acc *= old;
+            m = top;
+#pragma unroll
+            for (int b = 0; b < B; b++)
+                if (c0 + b * G < n) {
+                    const float f = exp2f(mm[b] - top);
+                    l += f * ll[b];
+                    acc += f * o[b];
+                }
+        }
+        float top = m;
+#pragma unroll
+        for (int x = L; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
+        float f = exp2f(m - top);
+        l *= f;
+        acc *= f;
+#pragma unroll
+        for (int x = L; x < 64; x <<= 1) {
+            l += __shfl_xor(l, x, 64);
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], x, 64);
-        const float f = 1.0f / sum;
-        if (g == 0) *reinterpret_cast<f32x4 *>(a.att + ((size_t)t.merge * heads + head) * D + d) = acc * f;
+        }
+        if constexpr (W > 1) {
+            if (lane < L) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) part[wave][d + e] = acc[e];
+                if (lane == 0) {
+                    part[wave][D] = top;
+                    part[wave][D + 1] = l;
+                }
+            }
+            __syncthreads();
+            float all = part[0][D];
+#pragma unroll
+            for (int x = 1; x < W; x++) all = fmaxf(all, part[x][D]);
+            l = 0.0f;
+            acc = f32x4{};
+#pragma unroll
+            for (int x = 0; x < W; x++) {
+                f = exp2f(part[x][D] - all);
+                l += f * part[x][D + 1];
+#pragma unroll
+                for (int e = 0; e < 4; e++) acc[e] += f * part[x][d + e];
+            }
+            __syncthreads();
+        }
+        f = 1.0f / l;
+        if (lane < L && (W == 1 || wave == 0))
+            *reinterpret_cast<f32x4 *>(a.att + ((size_t)t.merge * heads + head) * D + d) = acc * f;
     }
 }
 
@@ -502,11 +923,14 @@ struct AttendLaunch {
 };
 struct MergeLaunch {
     const BatchArgs &a;
-    int grid;
+    long long rows;
     hipStream_t s;
     template <int D, class T>
     hipError_t operator()() {
-        batch_merge_kernel<D><<<grid, 256, 0, s>>>(a);
+        if (a.max_states > 256 / D * 8)
+            batch_merge_kernel<D, 4><<<(int)std::min<long long>(1 << 20, rows), 256, 0, s>>>(a);
+        else
+            batch_merge_kernel<D, 1><<<(int)std::min<long long>(1 << 20, (rows + 3) / 4), 256, 0, s>>>(a);
         return hipGetLastError();
     }
 };
@@ -544,13 +968,6 @@ struct ReadLaunch {
         return hipGetLastError();
     }
 };
-struct Occupancy {
-    int blocks = 1;
-    template <int D, class T>
-    hipError_t operator()() {
-        return hipOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, batch_attend_kernel<D, T>, 256, 0);
-    }
-};
 
 }  // namespace
 
@@ -558,8 +975,7 @@ hipError_t launch_batch_attend(int head_dim, int bf16, const BatchArgs &a, int g
     return dispatch(head_dim, bf16, AttendLaunch{a, grid, s});
 }
 hipError_t launch_batch_merge(int head_dim, const BatchArgs &a, int merges, hipStream_t s) {
-    const long long waves = (long long)merges * a.group * a.kv_heads;
-    return dispatch(head_dim, 0, MergeLaunch{a, (int)std::min<long long>(1 << 20, (waves + 3) / 4), s});
+    return dispatch(head_dim, 0, MergeLaunch{a, (long long)merges * a.group * a.kv_heads, s});
 }
 hipError_t launch_batch_append(int head_dim, int bf16, const BatchAppendArgs &a, hipStream_t s) {
     return dispatch(head_dim, bf16, AppendLaunch{a, s});
@@ -571,10 +987,6 @@ hipError_t launch_batch_load(int head_dim, int bf16, const float *src, int src_c
 hipError_t launch_batch_read(int head_dim, int bf16, const void *src, int capacity, int kv_heads, int pos0, int n,
                              float *dst, hipStream_t s) {
     return dispatch(head_dim, bf16, ReadLaunch{src, capacity, kv_heads, pos0, n, dst, s});
-}
-int batch_blocks_per_cu(int head_dim, int bf16) {
-    Occupancy o;
-    return dispatch(head_dim, bf16, o) == hipSuccess && o.blocks > 0 ? o.blocks : 1;
 }
 
 }  // namespace wick

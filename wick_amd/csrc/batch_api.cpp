@@ -172,7 +172,7 @@ int set_up(wick_hip_batch *b) {
     b->lim.capacity = c.capacity;
     b->lim.prefix_capacity = c.prefix_capacity;
     b->lim.max_tokens = c.max_tokens;
-    b->lim.workgroups = prop.multiProcessorCount * wick::batch_blocks_per_cu(c.head_dim, c.type);
+    b->lim.cus = prop.multiProcessorCount;
     b->max_items = wick::batch_max_items(b->lim);
     b->state_rows = wick::batch_max_state_rows(b->lim);
     if (b->max_items * c.kv_heads > INT_MAX / 2 || b->state_rows > INT_MAX / 2)
@@ -408,13 +408,13 @@ int wick_hip_batch_attention_device(wick_hip_batch *b, int layer, const float *q
     a.kv_heads = c.kv_heads;
     a.shape = b->shape;
     a.total = b->head.total;
+    a.max_states = b->head.max_states;  // a captured call chooses by its own plan's
     a.scale = (float)(M_LOG2E / std::sqrt((double)c.head_dim));
     // a captured call serves later plans too: those may have more items, or states to join
     // where this one has none
     const bool later = capturing(b->stream);
-    int grid = b->head.items * c.kv_heads;
-    if (later && grid < b->lim.workgroups) grid = b->lim.workgroups;
-    HIP_TRY(wick::launch_batch_attend(c.head_dim, c.type, a, grid, b->stream));
+    const int items = later ? b->head.most_items : b->head.items;
+    HIP_TRY(wick::launch_batch_attend(c.head_dim, c.type, a, items * c.kv_heads, b->stream));
     const int merges = later ? b->head.total : b->head.merges;
     if (merges) HIP_TRY(wick::launch_batch_merge(c.head_dim, a, merges, b->stream));
     return WICK_HIP_OK;

@@ -20,6 +20,7 @@ struct BatchArgs {
     long long state_rows;
     int prefix_capacity, capacity, group, kv_heads, sequences, max_tokens;
     int shape, total;  // of the plan at the call
+    int max_states;    // most states of a row in it
     float scale;       // log2(e) / sqrt(D)
 };
 
@@ -44,8 +45,5 @@ hipError_t launch_batch_load(int head_dim, int bf16, const float *src, int src_c
 // dst [n][kv_heads * D] f32 from positions pos0.. of src [kv_heads][capacity][D].
 hipError_t launch_batch_read(int head_dim, int bf16, const void *src, int capacity, int kv_heads, int pos0, int n,
                              float *dst, hipStream_t s);
-
-// Resident workgroups of the attention kernel per CU.
-int batch_blocks_per_cu(int head_dim, int bf16);
 
 }  // namespace wick

@@ -3,10 +3,10 @@
 // A row is one (token, query head of a kv head's group) pair, numbered token * group +
 // head over the packed tokens; every kv head has the same rows and the same cut.  An
 // item is one workgroup's work for each kv head: a block of rows against a range of the
-// prefix's keys and a range of its sequence's own keys.
+// prefix's keys and a range of its sequence's own keys.  A block of up to 16 rows is
+// narrow (the four waves share the keys), one of up to 128 wide (the waves share the rows).
 //   whole items   rows of one sequence against all the keys that they see; att is
-//                 written directly.  For sequences with many rows, where such items
-//                 alone fill the GPU.
+//                 written directly.
 //   split items   the keys dealt to several items, each leaving partial states
 //                 (m, l, O) that a second launch joins.  The rows of all split
 //                 sequences together go against the prefix (a block's rows read a
@@ -21,14 +21,18 @@
 
 namespace wick {
 
-constexpr int kBatchRows = 32;   // rows of an item
-constexpr int kBatchStep = 128;  // keys a workgroup takes at a time: 4 waves x 32
+constexpr int kBatchRows = 16;   // rows of a narrow item
+constexpr int kBatchWide = 128;  // rows of a wide item: 4 waves x 32
+constexpr int kBatchStep = 128;  // keys a narrow item takes at a time: 4 waves x 32
+constexpr int kBatchFew = 48;    // rows up to which narrow items share them
+constexpr int kBatchBig = 64;    // rows from which a sequence is a candidate for whole items
 
 // One workgroup's work (device layout).
 struct BatchItem {
     int row0, nrows;   // rows [row0, row0 + nrows): of the packed tokens (seq >= 0) or of
                        // the split tokens (seq < 0, found through BatchToken::split)
-    int seq;           // sequence of the own keys; -1: prefix keys only
+    int seq;           // sequence of the own keys; -1: prefix keys only, split token i is packed
+                       // token i + shift; -2: prefix keys only, it is BatchToken::split of i
     int p0, p1;        // prefix keys
     int o0, o1;        // own keys; row r sees those up to r / group + shift
     int shift;
@@ -54,28 +58,31 @@ struct BatchHeader {
     int shape;           // wick_hip_batch_shape()
     int items, total, merges;
     int prefix_chunks, prefix_stride;  // state rows from one prefix chunk to the next
-    int pad[10];
+    int max_states;                    // most states of a row
+    int most_items;                    // of any plan for the same t
+    int pad[8];
 };
 static_assert(sizeof(BatchHeader) == 64, "");
 
 // What a handle was made for.
 struct BatchLimits {
     int group, kv_heads, sequences, capacity, prefix_capacity, max_tokens;
-    int workgroups;  // resident at once
+    int cus;  // the GPU's compute units
 };
 
-// Most items and state rows (per kv head) of any plan.  Split sequences have together at
-// most `workgroups` blocks of whole rows over all kv heads (with more they are whole) and one
-// ragged block each; their items are at most `workgroups` over all kv heads, or a block against
-// the prefix and one against its own keys where that is more.
+// Most items and state rows (per kv head) of any plan.  A sequence of kBatchBig rows or more
+// is split only where its longest item would cost twice the target, which the sum of its
+// items' costs (half the longest each, or more) allows for cus / kv_heads blocks
+// together; the others have less than kBatchBig rows each.
 inline int64_t batch_max_items(const BatchLimits &c) {
     const int64_t rows = (int64_t)c.max_tokens * c.group;
-    return 2 * (rows / kBatchRows + std::min(c.sequences, c.max_tokens) + 1) + c.workgroups / c.kv_heads + 1;
+    return 2 * (rows / kBatchRows + std::min(c.sequences, c.max_tokens) + 1) + c.cus / c.kv_heads + 1;
 }
 inline int64_t batch_max_state_rows(const BatchLimits &c) {
     const int64_t rows = (int64_t)c.max_tokens * c.group, few = std::min(c.sequences, c.max_tokens);
-    const int64_t blocks = std::min(rows / kBatchRows, (int64_t)c.workgroups / c.kv_heads + few) + few + 1;
-    return (2 * blocks + c.workgroups / c.kv_heads + 1) * kBatchRows;
+    const int64_t slots = c.cus / c.kv_heads + 1;
+    const int64_t split = std::min(rows, kBatchWide * slots + (kBatchBig + kBatchWide) * few);
+    return 2 * kBatchWide * slots + 2 * split + 2 * kBatchWide;
 }
 
 struct BatchPlan {
@@ -85,7 +92,19 @@ struct BatchPlan {
     int64_t state_rows = 0;
 };
 
-inline int batch_blocks(int64_t rows) { return (int)((rows + kBatchRows - 1) / kBatchRows); }
+constexpr double kPlanItem = 2.0;       // an item's cost besides its keys'
+constexpr double kPlanWhole = 2.0;      // targets that a whole item may cost
+constexpr double kPlanLeastWide = 4.0;  // least cost of a range of keys
+constexpr double kPlanLeastNarrow = 1.0;
+constexpr double kPlanShare = 1.0;      // compute units' shares of the sum that the target is one of
+
+// Cost of a block of `rows` rows against `keys` keys, in tiles of a wave: a wide item's waves
+// all take every 32 keys, a narrow one's every fourth; and what an item costs besides.
+inline double batch_cost(int64_t rows, int64_t keys) {
+    return keys / (rows > kBatchRows ? 32.0 : 128.0);
+}
+// Rows of a block where `rows` are cut into blocks.
+inline int batch_block(int64_t rows) { return rows <= kBatchFew ? kBatchRows : kBatchWide; }
 
 // The plan of a step; start and t as wick_hip_batch_plan has them, already checked.
 inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t, int prefix) {
@@ -94,61 +113,70 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
     for (int s = 0; s < c.sequences; s++) total += t[s];
     p.head.total = total;
     p.tokens.assign(total, BatchToken{});
-    int64_t whole_blocks = 0;
+    auto rows_of = [&](int s) { return (int64_t)t[s] * c.group; };
+    auto blocks = [](int64_t rows) { return (rows + batch_block(rows) - 1) / batch_block(rows); };
+    auto big = [&](int s) { return rows_of(s) >= kBatchBig; };
+
+    // what all items cost together, the big sequences in whole ones; the target is a
+    // compute unit's share
+    double sum = 0.0;
+    int64_t small_rows = 0;
     for (int s = 0; s < c.sequences; s++) {
-        const int64_t rows = (int64_t)t[s] * c.group;
-        if (rows >= kBatchRows) whole_blocks += batch_blocks(rows);
-    }
-    const bool wholes = whole_blocks * c.kv_heads >= c.workgroups;
-    auto whole = [&](int s) { return wholes && (int64_t)t[s] * c.group >= kBatchRows; };
-
-    // the split rows, and the shortest key range per item that keeps them within the
-    // resident workgroups
-    int splits = 0, longest = prefix;
-    for (int s = 0; s < c.sequences; s++)
-        if (!whole(s) && t[s] > 0) {
-            splits += t[s];
-            longest = std::max(longest, start[s] + t[s]);
+        const int64_t rows = rows_of(s);
+        if (big(s)) {
+            const double keys = (double)prefix + start[s] + 0.5 * t[s];
+            sum += blocks(rows) * (keys / 32.0 + kPlanItem);
+        } else if (rows) {
+            sum += blocks(rows) * (batch_cost(batch_block(rows), start[s] + t[s]) + kPlanItem);
+            small_rows += rows;
         }
-    const int64_t split_rows = (int64_t)splits * c.group;
-    auto chunks = [](int keys, int len) { return (keys + len - 1) / len; };
-    auto count = [&](int len) {
-        int64_t n = prefix ? (int64_t)batch_blocks(split_rows) * chunks(prefix, len) : 0;
-        for (int s = 0; s < c.sequences; s++)
-            if (!whole(s) && t[s] > 0)
-                n += (int64_t)batch_blocks((int64_t)t[s] * c.group) * chunks(start[s] + t[s], len);
-        return n;
-    };
-    const int64_t most = std::max(1, c.workgroups / c.kv_heads);
-    int lo = 1, hi = std::max(1, chunks(longest, kBatchStep));  // in steps
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (count(mid * kBatchStep) <= most)
-            hi = mid;
-        else
-            lo = mid + 1;
     }
-    const int len = lo * kBatchStep;
+    if (prefix && small_rows) sum += blocks(small_rows) * (batch_cost(batch_block(small_rows), prefix) + kPlanItem);
+    // no plan of the same t has more items: a block's ranges are at most its cost over the
+    // target and one more, the last rows' excess over the average another one
+    int64_t base = 0;
+    for (int s = 0; s < c.sequences; s++) base += 2 * blocks(rows_of(s)) + 1;
+    p.head.most_items = (int)std::min<int64_t>(batch_max_items(c), c.cus / c.kv_heads + 1 + 2 * base);
+    const double target = sum * c.kv_heads / (c.cus * kPlanShare);
+    auto whole = [&](int s) { return big(s) && batch_cost(kBatchWide, (int64_t)prefix + start[s] + t[s]) <= kPlanWhole * target; };
 
-    auto even = [&](int keys, int n) {  // n ranges over keys, in steps
-        return chunks(chunks(keys, n), kBatchStep) * kBatchStep;
+    // n even ranges over the keys of a block of `rows` rows, each near the target, in steps
+    auto range = [&](int64_t rows, int keys) {
+        const bool wide = batch_block(rows) == kBatchWide;
+        const double least = wide ? kPlanLeastWide : kPlanLeastNarrow;
+        const int n = std::max(1, (int)(batch_cost(batch_block(rows), keys) / std::max(target, least) + 0.999));
+        const int part = (keys + n - 1) / n;
+        const int step = wide ? 32 : kBatchStep;
+        return (part + step - 1) / step * step;
     };
-    if (prefix && splits) {
-        const int part = even(prefix, chunks(prefix, len)), n = chunks(prefix, part);
+    auto chunks = [](int keys, int len) { return (keys + len - 1) / len; };
+
+    int64_t split_rows = 0;
+    std::vector<int> split_token;
+    for (int s = 0, token = 0; s < c.sequences; token += t[s++])
+        if (!whole(s)) {
+            split_rows += rows_of(s);
+            for (int i = 0; i < t[s]; i++) split_token.push_back(token + i);
+        }
+    if (prefix && split_rows) {
+        const int part = range(split_rows, prefix), n = chunks(prefix, part), step = batch_block(split_rows);
         p.head.prefix_chunks = n;
         p.head.prefix_stride = (int)split_rows;
-        for (int k = 0; k < n; k++)
-            for (int64_t r = 0; r < split_rows; r += kBatchRows) {
+        for (int k = 0; k < n; k++) {
+            for (int64_t r = 0; r < split_rows; r += step) {
                 BatchItem it{};
                 it.row0 = (int)r;
-                it.nrows = (int)std::min<int64_t>(kBatchRows, split_rows - r);
-                it.seq = -1;
+                it.nrows = (int)std::min<int64_t>(step, split_rows - r);
+                const int first = (int)(r / c.group), end = (int)((r + it.nrows - 1) / c.group);
+                it.shift = split_token[first] - first;
+                it.seq = split_token[end] - end == it.shift ? -1 : -2;  // they ascend
                 it.p0 = k * part;
                 it.p1 = std::min(prefix, it.p0 + part);
                 it.state0 = (int)(p.state_rows + r);
                 p.items.push_back(it);
-                if (r + kBatchRows >= split_rows) p.state_rows += split_rows;
             }
+            p.state_rows += split_rows;
+        }
     }
     int token = 0, split = 0;
     for (int s = 0; s < c.sequences; s++) {
@@ -156,26 +184,26 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
             p.tokens[token + i].seq = s;
             p.tokens[token + i].pos = start[s] + i;
         }
-        const int keys = start[s] + t[s], rows = t[s] * c.group, shift = start[s] - token;
+        const int keys = start[s] + t[s], rows = (int)rows_of(s), shift = start[s] - token;
         const int64_t row0 = (int64_t)token * c.group;
+        const int step = batch_block(rows);
+        // rows [r, r + step) against own keys [o0, o1), as far as the last row sees them
         auto block = [&](int r, int o0, int o1, int64_t state0, int p1) {
             BatchItem it{};
             it.row0 = (int)(row0 + r);
-            it.nrows = std::min(kBatchRows, rows - r);
+            it.nrows = std::min(step, rows - r);
             it.seq = s;
             it.p1 = p1;
             it.o0 = o0;
-            // no key past the last one that the block's last row sees
             it.o1 = std::min(o1, (int)((row0 + r + it.nrows - 1) / c.group) + shift + 1);
-            it.o1 = std::max(it.o0, it.o1);
             it.shift = shift;
             it.state0 = (int)state0;
-            p.items.push_back(it);
+            if (it.o1 > it.o0) p.items.push_back(it);
         };
-        if (t[s] > 0 && whole(s)) {
-            for (int r = 0; r < rows; r += kBatchRows) block(r, 0, keys, -1, prefix);
-        } else if (t[s] > 0) {
-            const int part = even(keys, chunks(keys, len)), n = chunks(keys, part);
+        if (rows && whole(s)) {
+            for (int r = 0; r < rows; r += step) block(r, 0, keys, -1, prefix);
+        } else if (rows) {
+            const int part = range(rows, keys), n = chunks(keys, part);
             const bool direct = n == 1 && !prefix;
             for (int i = 0; i < t[s] && !direct; i++) {
                 BatchToken &m = p.tokens[split];
@@ -183,11 +211,12 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
                 m.prefix_state = split * c.group;
                 m.own_state = (int)(p.state_rows + (int64_t)i * c.group);
                 m.own_stride = rows;
-                m.own_chunks = n;
+                m.own_chunks = (start[s] + i) / part + 1;  // those in which it sees a key
+                p.head.max_states = std::max(p.head.max_states, p.head.prefix_chunks + m.own_chunks);
                 split++;
             }
             for (int k = 0; k < n; k++) {
-                for (int r = 0; r < rows; r += kBatchRows)
+                for (int r = 0; r < rows; r += step)
                     block(r, k * part, std::min(keys, (k + 1) * part), direct ? -1 : p.state_rows + r, 0);
                 if (!direct) p.state_rows += rows;
             }
@@ -195,10 +224,12 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
         token += t[s];
     }
     p.head.merges = split;
-    // the longest items first
+    // the costliest items first
     std::stable_sort(p.items.begin(), p.items.end(), [](const BatchItem &a, const BatchItem &b) {
-        const int x = a.p1 - a.p0 + a.o1 - a.o0, y = b.p1 - b.p0 + b.o1 - b.o0;
-        return x / kBatchStep > y / kBatchStep;
+        const auto cost = [](const BatchItem &x) {
+            return (int)batch_cost(x.nrows, (int64_t)x.p1 - x.p0 + x.o1 - x.o0);
+        };
+        return cost(a) > cost(b);
     });
     p.head.items = (int)p.items.size();
     return p;

@@ -74,4 +74,12 @@ __device__ __forceinline__ float rows_sum(float v) {
     return __uint_as_float(p[0]) + __uint_as_float(p[1]);
 }
 
+// Maximum of the same 4 lanes.
+__device__ __forceinline__ float rows_max(float v) {
+    auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+}
+
 }  // namespace wick
