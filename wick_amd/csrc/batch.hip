@@ -172,6 +172,13 @@ __device__ __forceinline__ void parts4(const __bf16 *x, b16x4 (&part)[1]) {
     for (int i = 0; i < 4; i++) part[0][i] = x[i];
 }
 
+// x / d for 0 <= x < 2^31, inv = min(2^32 / d rounded up, 2^32 - 1): off by one at most before the correction.
+__device__ __forceinline__ int divide(int x, int d, unsigned inv) {
+    int q = (int)__umulhi((unsigned)x, inv);
+    const int r = x - q * d;
+    return r < 0 ? q - 1 : r >= d ? q + 1 : q;
+}
+
 __device__ __forceinline__ float other_half(float v) {
     const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float((threadIdx.x & 32) ? p[0] : p[1]);
@@ -421,10 +428,12 @@ template <int D, class T>
 struct Few {
     using S = Shape<D, T>;
     static constexpr int KS = S::KS16, NB = S::NB16;
+    // a step's keys and values are requested a step ahead where there are registers for both
+    static constexpr int AHEAD = D * sizeof(T) <= 256 ? 2 : 1;
     Parts<3> q[KS];
     f32x4 o[NB];
     float m, l;
-    T k[2][KS][8], v[8][NB];
+    T k[AHEAD][2][KS][8], v[AHEAD][8][NB];
 
     __device__ __forceinline__ void begin(const float *src, float scale, int quad) {
 #pragma unroll
@@ -442,31 +451,31 @@ struct Few {
     }
 
     // of n keys left at p
-    __device__ __forceinline__ void load_k(const T *p, int n, int col, int quad) {
+    __device__ __forceinline__ void load_k(int to, const T *p, int n, int col, int quad) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const unsigned at = min(16 * u + col, n - 1) * D + 8 * (D >= 32 ? quad : quad & 1);
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) load_n<8>(p + 32 * ks + at, k[u][ks]);
+            for (int ks = 0; ks < KS; ks++) load_n<8>(p + 32 * ks + at, k[to][u][ks]);
         }
     }
-    __device__ __forceinline__ void load_v(const T *p, int n, int col, int quad) {
+    __device__ __forceinline__ void load_v(int to, const T *p, int n, int col, int quad) {
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            load_n<NB>(p + (unsigned)(min(16 * (j / 4) + 4 * quad + j % 4, n - 1) * D + NB * col), v[j]);
+            load_n<NB>(p + (unsigned)(min(16 * (j / 4) + 4 * quad + j % 4, n - 1) * D + NB * col), v[to][j]);
     }
 
-    __device__ __forceinline__ void scores(f32x4 (&s)[2]) const {
+    __device__ __forceinline__ void scores(int at, f32x4 (&s)[2]) const {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             s[u] = f32x4{};
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) s[u] = product(parts8(k[u][ks]), q[ks], s[u]);  // 16 dimensions: q's rest is 0
+            for (int ks = 0; ks < KS; ks++) s[u] = product(parts8(k[at][u][ks]), q[ks], s[u]);  // 16 dimensions: q's rest is 0
         }
     }
 
     // keys past `left` of the 32 are hidden
-    __device__ __forceinline__ void values(f32x4 (&s)[2], bool mask, int left) {
+    __device__ __forceinline__ void values(int at, f32x4 (&s)[2], bool mask, int left) {
         if (mask) {
 #pragma unroll
             for (int i = 0; i < 8; i++) s[i / 4][i % 4] = 16 * (i / 4) + i % 4 > left ? -INFINITY : s[i / 4][i % 4];
@@ -493,7 +502,7 @@ struct Few {
         for (int b = 0; b < NB; b++) {
             T y[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = v[j][b];
+            for (int j = 0; j < 8; j++) y[j] = v[at][j][b];
             o[b] = product(parts8(y), w, o[b]);
         }
     }
@@ -524,8 +533,8 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
     }
     if ((int)blockIdx.x >= work) return;
     {
-        const BatchItem it = a.items[blockIdx.x / a.kv_heads];
-        const int kh = blockIdx.x % a.kv_heads;
+        const int item = divide(blockIdx.x, a.kv_heads, a.inv_kv_heads), kh = blockIdx.x - item * a.kv_heads;
+        const BatchItem it = a.items[item];
         const T *pk = static_cast<const T *>(a.pk) + (size_t)kh * a.prefix_capacity * D;
         const T *pv = static_cast<const T *>(a.pv) + (size_t)kh * a.prefix_capacity * D;
         const size_t own = it.seq < 0 ? 0 : ((size_t)it.seq * a.kv_heads + kh) * a.capacity * D;
@@ -534,11 +543,11 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
 
         // row r of the item: its place in q and att, its last own key, its states
         auto row_at = [&](int r) {
-            const int row = it.row0 + r, t = row / a.group, h = row - t * a.group;
+            const int row = it.row0 + r, t = divide(row, a.group, a.inv_group), h = row - t * a.group;
             const int token = it.seq >= 0 ? t : it.seq == -1 ? t + it.shift : a.tokens[t].split;
             return ((size_t)token * heads + kh * a.group + h) * D;
         };
-        auto last_of = [&](int r) { return it.seq < 0 ? -1 : (it.row0 + r) / a.group + it.shift; };
+        auto last_of = [&](int r) { return it.seq < 0 ? -1 : divide(it.row0 + r, a.group, a.inv_group) + it.shift; };
         auto state_at = [&](int r) { return (size_t)kh * a.state_rows + it.state0 + r; };
         auto redo = [&](int r) {
             const size_t at = direct ? 0 : state_at(r);
@@ -581,7 +590,7 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
             load_k(min(1, tiles - 1));  // past the last tile the last one again: no one reads it
             __syncthreads();
             // a tile for this wave; MASK: some of its keys are past the end or hidden from some rows
-            auto tile = [&](auto mask, int t, int tile0, int seen) {
+            auto tile = [&](auto mask, int t, int tile0, int seen, bool second) {
                 constexpr bool MASK = decltype(mask)::value;
                 f32x16 s[KT / 32];
                 {
@@ -603,6 +612,11 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
                 constexpr int G = 2 * NB, UNITS = sk.UNITS * 32 / KT;  // of a 32-key part
 #pragma unroll
                 for (int sub = 0; sub < KT / 32; sub++) {
+                    if (MASK && sub > 0 && !second) {  // no key of it is seen
+#pragma unroll
+                        for (int i = 0; i < UNITS; i++) sk.store(sub * UNITS + i, kat, wave);
+                        break;
+                    }
                     Parts<S::KP> x = read(lds.tile.v, sub * G, lane), y;
                     st.template scores<MASK>(s[sub], tile0 + 32 * sub, half, seen);
                     Parts<3> w8[2];
@@ -636,9 +650,10 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
                 const int any = max(0, (part ? min(end, end_last + 1) : end) - begin);
                 if (nr <= 0) break;
                 const int t0 = t;
-                for (const int stop = t0 + all / KT; t < stop; t++) tile(std::false_type{}, t, 0, 0);
+                for (const int stop = t0 + all / KT; t < stop; t++) tile(std::false_type{}, t, 0, 0, true);
                 for (const int stop = t0 + (any + KT - 1) / KT; t < stop; t++)
-                    tile(std::true_type{}, t, begin + (t - t0) * KT, part ? min(last, end - 1) : end - 1);
+                    tile(std::true_type{}, t, begin + (t - t0) * KT, part ? min(last, end - 1) : end - 1,
+                         any - (t - t0) * KT > 32);
             }
             for (; t < tiles; t++) {
 #pragma unroll
@@ -692,21 +707,40 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
             const int tiles = np + max(0, (it.o1 - it.o0 - 32 * wave + 127) / 128);
             auto first_key = [&](int t) { return 32 * wave + (t < np ? it.p0 + 128 * t : it.o0 + 128 * (t - np)); };
             Few<D, T> st;
-            auto load_k = [&](int t) {
-                const int key = first_key(t);
-                st.load_k((t < np ? pk : ok) + (size_t)key * D, (t < np ? it.p1 : it.o1) - key, c, quad);
+            constexpr int AHEAD = Few<D, T>::AHEAD;
+            // past the last tile the last one again
+            auto load_k = [&](int to, int t) {
+                const int u = min(t, tiles - 1), key = first_key(u);
+                st.load_k(to, (u < np ? pk : ok) + (size_t)key * D, (u < np ? it.p1 : it.o1) - key, c, quad);
             };
-            if (tiles > 0) load_k(0);
+            auto load_v = [&](int to, int t) {
+                const int u = min(t, tiles - 1), key = first_key(u);
+                st.load_v(to, (u < np ? pv : ov) + (size_t)key * D, (u < np ? it.p1 : it.o1) - key, c, quad);
+            };
+            if (tiles > 0) {
+                load_k(0, 0);
+                if (AHEAD == 2) load_v(0, 0);
+            }
             st.begin(a.q + row_at(r), a.scale, quad);
-            for (int t = 0; t < tiles; t++) {
-                const bool o = t >= np;
-                const int key0 = first_key(t), end = o ? it.o1 : it.p1;
-                st.load_v((o ? ov : pv) + (size_t)key0 * D, end - key0, c, quad);
-                f32x4 s[2];
-                st.scores(s);
-                load_k(min(t + 1, tiles - 1));  // past the last tile the last one again
-                st.values(s, key0 + 32 > end || (o && key0 + 31 > first_last),
-                          (o ? min(last, end - 1) : end - 1) - key0 - 4 * quad);
+            for (int t0 = 0; t0 < tiles; t0 += AHEAD) {
+#pragma unroll
+                for (int x = 0; x < AHEAD; x++) {
+                    const int t = t0 + x;
+                    if (x > 0 && t >= tiles) break;
+                    if (AHEAD == 2) {
+                        load_k(1 - x, t + 1);
+                        load_v(1 - x, t + 1);
+                    } else {
+                        load_v(0, t);
+                    }
+                    f32x4 s[2];
+                    st.scores(x, s);
+                    if (AHEAD == 1) load_k(0, t + 1);
+                    const bool o = t >= np;
+                    const int key0 = first_key(t), end = o ? it.o1 : it.p1;
+                    st.values(x, s, key0 + 32 > end || (o && key0 + 31 > first_last),
+                              (o ? min(last, end - 1) : end - 1) - key0 - 4 * quad);
+                }
             }
             const float l = rows_sum(st.l);
             // join the waves' states: O by row through LDS
@@ -735,7 +769,7 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
         for (int e = 0; e < E; e++) acc[e] = 0.0f;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float f = exp2f(j.m[i][row] - to);
+            const float f = __builtin_amdgcn_exp2f(j.m[i][row] - to);
             sum += f * j.l[i][row];
 #pragma unroll
             for (int e = 0; e < E; e++) acc[e] += f * j.o[i][row][d0 + e];
@@ -774,7 +808,8 @@ __global__ __launch_bounds__(256) void batch_merge_kernel(BatchArgs a) {
     const int work = a.head->merges * heads, prefix_chunks = a.head->prefix_chunks, stride = a.head->prefix_stride;
     constexpr int R = 4 / W;  // rows of a workgroup
     for (int w = blockIdx.x * R + (W > 1 ? 0 : wave); w < work; w += gridDim.x * R) {
-        const int i = w / heads, head = w - i * heads, kh = head / a.group, h = head - kh * a.group;
+        const int i = divide(w, heads, a.inv_heads), head = w - i * heads, kh = divide(head, a.group, a.inv_group),
+                  h = head - kh * a.group;
         const BatchToken t = a.tokens[i];
         const size_t base = (size_t)kh * a.state_rows + h;
         const int n = prefix_chunks + t.own_chunks;

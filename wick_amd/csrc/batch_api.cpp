@@ -406,6 +406,9 @@ int wick_hip_batch_attention_device(wick_hip_batch *b, int layer, const float *q
     a.capacity = c.capacity;
     a.group = b->lim.group;
     a.kv_heads = c.kv_heads;
+    a.inv_group = wick::batch_inverse(a.group);
+    a.inv_kv_heads = wick::batch_inverse(a.kv_heads);
+    a.inv_heads = wick::batch_inverse(c.heads);
     a.shape = b->shape;
     a.total = b->head.total;
     a.max_states = b->head.max_states;  // a captured call chooses by its own plan's

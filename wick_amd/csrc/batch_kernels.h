@@ -18,11 +18,17 @@ struct BatchArgs {
     const BatchItem *items;
     float *po, *pm, *pl;  // states: [kv_heads][state_rows] x D, 1, 1
     long long state_rows;
-    int prefix_capacity, capacity, group, kv_heads, sequences, max_tokens;
+    int prefix_capacity, capacity, group, kv_heads;
+    unsigned inv_group, inv_kv_heads, inv_heads;  // batch_inverse of group, kv_heads and their product
     int shape, total;  // of the plan at the call
     int max_states;    // most states of a row in it
     float scale;       // log2(e) / sqrt(D)
 };
+
+// For the kernels' divisions by d >= 1.
+inline unsigned batch_inverse(int d) {
+    return d == 1 ? 0xffffffffu : (unsigned)(((1ull << 32) + d - 1) / d);
+}
 
 // The planned tokens' attention: `grid` workgroups over the items of every kv head.
 hipError_t launch_batch_attend(int head_dim, int bf16, const BatchArgs &a, int grid, hipStream_t s);

@@ -25,7 +25,6 @@ constexpr int kBatchRows = 16;   // rows of a narrow item
 constexpr int kBatchWide = 128;  // rows of a wide item: 4 waves x 32
 constexpr int kBatchStep = 128;  // keys a narrow item takes at a time: 4 waves x 32
 constexpr int kBatchFew = 48;    // rows up to which narrow items share them
-constexpr int kBatchBig = 64;    // rows from which a sequence is a candidate for whole items
 
 // One workgroup's work (device layout).
 struct BatchItem {
@@ -70,19 +69,20 @@ struct BatchLimits {
     int cus;  // the GPU's compute units
 };
 
-// Most items and state rows (per kv head) of any plan.  A sequence of kBatchBig rows or more
-// is split only where its longest item would cost twice the target, which the sum of its
-// items' costs (half the longest each, or more) allows for cus / kv_heads blocks
-// together; the others have less than kBatchBig rows each.
+// Most items and state rows (per kv head) of any plan.  A big sequence is split only where
+// its longest item costs more than 1 / kPlanLone of a unit's share, and its items cost half the
+// longest each or more, so that the split ones have at most 2.6 cus / kv_heads blocks together;
+// steps without wide blocks have fewer than cus / kv_heads of them; other sequences have up to
+// kBatchFew rows.  Ranges of a block are at most its cost over the target and one more.
 inline int64_t batch_max_items(const BatchLimits &c) {
     const int64_t rows = (int64_t)c.max_tokens * c.group;
-    return 2 * (rows / kBatchRows + std::min(c.sequences, c.max_tokens) + 1) + c.cus / c.kv_heads + 1;
+    return 2 * (rows / kBatchRows + std::min(c.sequences, c.max_tokens) + 1) + 2 * c.cus / c.kv_heads + 1;
 }
 inline int64_t batch_max_state_rows(const BatchLimits &c) {
     const int64_t rows = (int64_t)c.max_tokens * c.group, few = std::min(c.sequences, c.max_tokens);
     const int64_t slots = c.cus / c.kv_heads + 1;
-    const int64_t split = std::min(rows, kBatchWide * slots + (kBatchBig + kBatchWide) * few);
-    return 2 * kBatchWide * slots + 2 * split + 2 * kBatchWide;
+    const int64_t split = std::min(rows, 3 * kBatchWide * slots + (kBatchFew + kBatchWide) * few);
+    return 6 * kBatchWide * slots + 2 * split + 2 * kBatchWide;
 }
 
 struct BatchPlan {
@@ -93,18 +93,18 @@ struct BatchPlan {
 };
 
 constexpr double kPlanItem = 2.0;       // an item's cost besides its keys'
-constexpr double kPlanWhole = 2.0;      // targets that a whole item may cost
+constexpr double kPlanJoin = 18.0;      // what leaving states and joining them costs a step
+constexpr double kPlanLone = 1.3;       // a tile's cost where a unit has one wide item, not two
 constexpr double kPlanLeastWide = 4.0;  // least cost of a range of keys
 constexpr double kPlanLeastNarrow = 1.0;
-constexpr double kPlanShare = 1.0;      // compute units' shares of the sum that the target is one of
+constexpr double kPlanAlone = 3.0;      // up to which ranges are not cut to save the second launch
+constexpr double kPlanWideItems = 2.0;  // wide items to cut for each compute unit (narrow ones: one)
 
 // Cost of a block of `rows` rows against `keys` keys, in tiles of a wave: a wide item's waves
 // all take every 32 keys, a narrow one's every fourth; and what an item costs besides.
 inline double batch_cost(int64_t rows, int64_t keys) {
     return keys / (rows > kBatchRows ? 32.0 : 128.0);
 }
-// Rows of a block where `rows` are cut into blocks.
-inline int batch_block(int64_t rows) { return rows <= kBatchFew ? kBatchRows : kBatchWide; }
 
 // The plan of a step; start and t as wick_hip_batch_plan has them, already checked.
 inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t, int prefix) {
@@ -114,43 +114,67 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
     p.head.total = total;
     p.tokens.assign(total, BatchToken{});
     auto rows_of = [&](int s) { return (int64_t)t[s] * c.group; };
-    auto blocks = [](int64_t rows) { return (rows + batch_block(rows) - 1) / batch_block(rows); };
-    auto big = [&](int s) { return rows_of(s) >= kBatchBig; };
+    auto chunks = [](int64_t keys, int64_t len) { return (keys + len - 1) / len; };
 
-    // what all items cost together, the big sequences in whole ones; the target is a
-    // compute unit's share
+    // Wide blocks where, cut as finely as they may be, they give every compute unit an
+    // item; narrow ones in smaller steps, which are eight times as many.
+    int64_t most_wide = 0, small_rows = 0;
+    for (int s = 0; s < c.sequences; s++) {
+        const int64_t rows = rows_of(s), keys = (int64_t)start[s] + t[s];
+        if (rows > kBatchFew)
+            most_wide += chunks(rows, kBatchWide) * chunks(prefix + keys, (int64_t)(32 * kPlanLeastWide));
+        else
+            small_rows += rows;
+    }
+    if (small_rows > kBatchFew)
+        most_wide += chunks(small_rows, kBatchWide) * chunks(prefix, (int64_t)(32 * kPlanLeastWide));
+    const bool wides = most_wide * c.kv_heads >= c.cus;
+    auto block_of = [&](int64_t rows) { return wides && rows > kBatchFew ? kBatchWide : kBatchRows; };
+    auto blocks = [&](int64_t rows) { return chunks(rows, block_of(rows)); };
+    auto big = [&](int s) { return block_of(rows_of(s)) == kBatchWide; };
+
+    // what all items cost together, the big sequences in whole ones; a compute unit's share
+    // of it is what the step takes at best
     double sum = 0.0;
-    int64_t small_rows = 0;
+    // Few keys for every sequence that is not big: each takes all of its own, the prefix
+    // again and again, which costs less than the second launch
+    double alone_most = 0.0, alone_sum = 0.0;
+    // no plan of the same t has more items: a block's ranges are at most its cost over the
+    // target and one more, the last rows' excess over the average another one
+    int64_t base = 0;
+    small_rows = 0;
     for (int s = 0; s < c.sequences; s++) {
         const int64_t rows = rows_of(s);
         if (big(s)) {
             const double keys = (double)prefix + start[s] + 0.5 * t[s];
             sum += blocks(rows) * (keys / 32.0 + kPlanItem);
         } else if (rows) {
-            sum += blocks(rows) * (batch_cost(batch_block(rows), start[s] + t[s]) + kPlanItem);
+            sum += blocks(rows) * (batch_cost(kBatchRows, start[s] + t[s]) + kPlanItem);
             small_rows += rows;
+            const double cost = batch_cost(kBatchRows, (int64_t)prefix + start[s] + t[s]);
+            alone_most = std::max(alone_most, cost);
+            alone_sum += blocks(rows) * (cost + kPlanItem);
         }
+        base += 2 * chunks(rows, kBatchRows) + 1;
     }
-    if (prefix && small_rows) sum += blocks(small_rows) * (batch_cost(batch_block(small_rows), prefix) + kPlanItem);
-    // no plan of the same t has more items: a block's ranges are at most its cost over the
-    // target and one more, the last rows' excess over the average another one
-    int64_t base = 0;
-    for (int s = 0; s < c.sequences; s++) base += 2 * blocks(rows_of(s)) + 1;
-    p.head.most_items = (int)std::min<int64_t>(batch_max_items(c), c.cus / c.kv_heads + 1 + 2 * base);
-    const double target = sum * c.kv_heads / (c.cus * kPlanShare);
-    auto whole = [&](int s) { return big(s) && batch_cost(kBatchWide, (int64_t)prefix + start[s] + t[s]) <= kPlanWhole * target; };
+    if (prefix && small_rows)
+        sum += blocks(small_rows) * (batch_cost(block_of(small_rows), prefix) + kPlanItem);
+    const double share = sum * c.kv_heads / c.cus, target = wides ? share / kPlanWideItems : share;
+    p.head.most_items = (int)std::min<int64_t>(batch_max_items(c), 2 * c.cus / c.kv_heads + 1 + 2 * base);
+    const bool alone = alone_most <= kPlanAlone && alone_sum * c.kv_heads <= kPlanAlone * c.cus;
+    auto whole = [&](int s) {
+        return big(s) ? kPlanLone * batch_cost(kBatchWide, (int64_t)prefix + start[s] + t[s]) <= share + kPlanJoin : alone;
+    };
 
     // n even ranges over the keys of a block of `rows` rows, each near the target, in steps
     auto range = [&](int64_t rows, int keys) {
-        const bool wide = batch_block(rows) == kBatchWide;
+        const bool wide = block_of(rows) == kBatchWide;
         const double least = wide ? kPlanLeastWide : kPlanLeastNarrow;
-        const int n = std::max(1, (int)(batch_cost(batch_block(rows), keys) / std::max(target, least) + 0.999));
+        const int n = std::max(1, (int)(batch_cost(block_of(rows), keys) / std::max(target, least) + 0.999));
         const int part = (keys + n - 1) / n;
         const int step = wide ? 32 : kBatchStep;
         return (part + step - 1) / step * step;
     };
-    auto chunks = [](int keys, int len) { return (keys + len - 1) / len; };
-
     int64_t split_rows = 0;
     std::vector<int> split_token;
     for (int s = 0, token = 0; s < c.sequences; token += t[s++])
@@ -159,7 +183,7 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
             for (int i = 0; i < t[s]; i++) split_token.push_back(token + i);
         }
     if (prefix && split_rows) {
-        const int part = range(split_rows, prefix), n = chunks(prefix, part), step = batch_block(split_rows);
+        const int part = range(split_rows, prefix), n = (int)chunks(prefix, part), step = block_of(split_rows);
         p.head.prefix_chunks = n;
         p.head.prefix_stride = (int)split_rows;
         for (int k = 0; k < n; k++) {
@@ -186,7 +210,7 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
         }
         const int keys = start[s] + t[s], rows = (int)rows_of(s), shift = start[s] - token;
         const int64_t row0 = (int64_t)token * c.group;
-        const int step = batch_block(rows);
+        const int step = block_of(rows);
         // rows [r, r + step) against own keys [o0, o1), as far as the last row sees them
         auto block = [&](int r, int o0, int o1, int64_t state0, int p1) {
             BatchItem it{};
@@ -203,7 +227,7 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
         if (rows && whole(s)) {
             for (int r = 0; r < rows; r += step) block(r, 0, keys, -1, prefix);
         } else if (rows) {
-            const int part = range(rows, keys), n = chunks(keys, part);
+            const int part = range(rows, keys), n = (int)chunks(keys, part);
             const bool direct = n == 1 && !prefix;
             for (int i = 0; i < t[s] && !direct; i++) {
                 BatchToken &m = p.tokens[split];

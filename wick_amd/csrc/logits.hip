@@ -19,13 +19,14 @@ constexpr uint32_t kSeen = 0x80000000u;
 // rows of any alignment: 4 values, aligned as one
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4u __attribute__((ext_vector_type(4), aligned(4)));
 
 template <int SLAB>
 __global__ __launch_bounds__(kT) void logits_kernel(LogitArgs a) {
 #pragma clang fp contract(off)
     constexpr int U = SLAB / (4 * kT);  // passes of 4 ids a thread
-    __shared__ uint32_t count[SLAB];    // times among the generated tokens, and kSeen
-    __shared__ uint32_t bias[SLAB];     // 1 + the number of the id's last bias entry
+    // first times among the generated tokens, and kSeen; then 1 + the number of the last bias
+    __shared__ uint32_t note[SLAB];
     const int tid = threadIdx.x, row = blockIdx.x / a.slabs, s0 = (blockIdx.x - row * a.slabs) * SLAB;
     const wick_hip_logit_rules &r = a.r;
     const float *x = a.x + (size_t)row * a.stride;
@@ -61,41 +62,57 @@ __global__ __launch_bounds__(kT) void logits_kernel(LogitArgs a) {
         b0 = min(max(r.bias_start[row], 0), r.n_bias);
         b1 = min(max(r.bias_start[row + 1], 0), r.n_bias);
     }
-    const bool rules = n > 0 || b1 > b0;
-    if (rules) {
+    u4 *const mine = reinterpret_cast<u4 *>(note) + tid;  // mine[u * kT]: this thread's ids of pass u
+    if (n > 0) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            reinterpret_cast<u4 *>(count)[tid + u * kT] = u4{0, 0, 0, 0};
-            reinterpret_cast<u4 *>(bias)[tid + u * kT] = u4{0, 0, 0, 0};
-        }
+        for (int u = 0; u < U; u++) mine[u * kT] = u4{0, 0, 0, 0};
         __syncthreads();
         const uint32_t *tokens = r.tokens + (size_t)row * r.tokens_stride;
-        for (int i = tid; i < n; i += kT) {
-            const uint32_t at = tokens[i] - (uint32_t)s0;
+        auto seen = [&](int i, uint32_t id) {
+            const uint32_t at = id - (uint32_t)s0;
             if (at < (uint32_t)SLAB) {
-                atomicOr(&count[at], kSeen);
-                if (i >= prompt) atomicAdd(&count[at], 1u);
+                atomicOr(&note[at], kSeen);
+                if (i >= prompt) atomicAdd(&note[at], 1u);
             }
+        };
+        const int n4 = n & ~3;
+        for (int i = 4 * tid; i < n4; i += 4 * kT) {
+            const u4u id = *reinterpret_cast<const u4u *>(tokens + i);
+#pragma unroll
+            for (int j = 0; j < 4; j++) seen(i + j, id[j]);
         }
-        for (int i = b0 + tid; i < b1; i += kT) {
-            const uint32_t at = r.bias_ids[i] - (uint32_t)s0;
-            if (at < (uint32_t)SLAB) atomicMax(&bias[at], (uint32_t)(i - b0) + 1);
-        }
+        if (n4 + tid < n) seen(n4 + tid, tokens[n4 + tid]);
         __syncthreads();
         const float rep = r.repetition ? r.repetition[row] : 1.0f, pres = r.presence ? r.presence[row] : 0.0f,
                     freq = r.frequency ? r.frequency[row] : 0.0f;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const u4 c = reinterpret_cast<const u4 *>(count)[tid + u * kT], b = reinterpret_cast<const u4 *>(bias)[tid + u * kT];
+            const u4 c = mine[u * kT];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 float y = v[u][j];
                 if (c[j]) y = y > 0.0f ? y / rep : y * rep;
                 const uint32_t times = c[j] & ~kSeen;
                 if (times) y -= freq * (float)times + pres;
-                if (b[j]) y += r.bias[b0 + b[j] - 1];
                 v[u][j] = y;
             }
+        }
+    }
+    if (b1 > b0) {  // a thread clears its own ids, which only it has read
+#pragma unroll
+        for (int u = 0; u < U; u++) mine[u * kT] = u4{0, 0, 0, 0};
+        __syncthreads();
+        for (int i = b0 + tid; i < b1; i += kT) {
+            const uint32_t at = r.bias_ids[i] - (uint32_t)s0;
+            if (at < (uint32_t)SLAB) atomicMax(&note[at], (uint32_t)(i - b0) + 1);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const u4 c = mine[u * kT];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (c[j]) v[u][j] += r.bias[b0 + c[j] - 1];
         }
     }
 #pragma unroll
