@@ -1,7 +1,7 @@
 /*
  * wick_hip_batch.h -- several sequences at once over one shared prefix, on the GPU.
  *
- * wick serves one sequence per Session (/root/reference/src/engine.rs:101-139) and
+ * wick serves one sequence per Session (src/engine.rs:101-139) and
  * keeps a prompt's positions when the next prompt begins with them (:127-132).  A
  * batch is that idea for many sequences at a time: one prefix (a system prompt, a
  * document) that all of them continue, its keys and values held and read once for
@@ -15,7 +15,7 @@
  * sequence 0's tokens, then those of sequence 1, with no gaps.
  *
  * Token i of sequence s, at its position start[s] + i behind the prefix, attends as
- * Model::attention (/root/reference/src/model.rs:518-553) does to a context of the
+ * Model::attention (src/model.rs:518-553) does to a context of the
  * prefix followed by the sequence's positions 0..=start[s]+i:
  *   att = softmax(q . k / sqrt(head_dim)) v.
  * q and att are f32.  The caches hold f32 (WICK_HIP_BATCH_F32) or bfloat16

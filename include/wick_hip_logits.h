@@ -2,7 +2,7 @@
  * wick_hip_logits.h -- penalties, biases and grammar masks on a batch's logits, on the GPU.
  *
  * wick's sampler has a repetition penalty for one sequence
- * (/root/reference/src/sampler.rs:75-83).  This is that step for a batch, each row with
+ * (src/sampler.rs:75-83).  This is that step for a batch, each row with
  * its own settings, and what serving programs put next to it: presence and frequency
  * penalties, biases on single ids, and grammars that allow a part of the vocabulary.  The
  * rows that come out go to wick_hip_sampler_sample_device or any other draw.

@@ -19,6 +19,7 @@ GOOD = dict(layers=1, heads=4, kv_heads=2, head_dim=64, sequences=2, capacity=16
     (dict(type=2), "type"), (dict(capacity=(1 << 30) + 1, max_tokens=1), "2^30"),
     (dict(prefix_capacity=(1 << 30) + 1), "2^30"), (dict(max_tokens=33), "max_tokens"),
     (dict(heads=1 << 20, capacity=1 << 20, max_tokens=1 << 20), "2^30"),
+    (dict(heads=65536, kv_heads=65536), "65535"),
 ])
 def test_create_refuses(change, says):
     lib = _native.load()
@@ -69,7 +70,7 @@ def test_unknown_type_name():
 
 @pytest.mark.parametrize("rules,call,says", [
     (None, {}, "null"), ({}, dict(logits=None), "null"), ({}, dict(out=None), "null"), ({}, dict(rows=-1), "rows"),
-    ({}, dict(vocab=0), "vocab"), ({}, dict(stride=7), "strides"), ({}, dict(out_stride=7), "strides"),
+    ({}, dict(vocab=0), "vocab"), ({}, dict(vocab=(1 << 30) + 1), "2^30"), ({}, dict(stride=7), "strides"), ({}, dict(out_stride=7), "strides"),
     (dict(tokens=4096), {}, "n_tokens"), (dict(tokens_stride=-1), {}, "tokens_stride"), (dict(n_bias=-1), {}, "n_bias"),
     (dict(bias=4096, bias_ids=4096), {}, "bias_start"), (dict(bias=4096, bias_start=4096), {}, "bias_ids"),
     (dict(mask=4096), {}, "masks"), (dict(mask=4096, masks=1), dict(rows=2), "masks"),

@@ -1,8 +1,8 @@
 """ctypes wrapper of include/wick_hip_batch.h: several sequences over one shared prefix.
 
-wick keeps one sequence's prompt prefix (/root/reference/src/engine.rs:127-132);
+wick keeps one sequence's prompt prefix (src/engine.rs:127-132);
 DeviceBatch holds one prefix for many sequences and attends for all of them at once, as
-Model::attention (/root/reference/src/model.rs:518-553) does for each.
+Model::attention (src/model.rs:518-553) does for each.
 """
 import ctypes
 

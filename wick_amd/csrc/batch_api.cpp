@@ -122,6 +122,7 @@ int check_config(const wick_hip_batch_config &c) {
         return set_error(WICK_HIP_EINVAL, "layers, kv_heads, sequences, capacity and max_tokens must be >= 1");
     if (c.heads < 1 || c.heads % c.kv_heads != 0)
         return set_error(WICK_HIP_EINVAL, "heads (%d) must be a positive multiple of kv_heads (%d)", c.heads, c.kv_heads);
+    if (c.kv_heads > 65535) return set_error(WICK_HIP_EINVAL, "kv_heads must be at most 65535");
     if (c.head_dim != 16 && c.head_dim != 32 && c.head_dim != 64 && c.head_dim != 128)
         return set_error(WICK_HIP_EINVAL, "head_dim %d not supported (16, 32, 64, 128)", c.head_dim);
     if (c.prefix_capacity < 0) return set_error(WICK_HIP_EINVAL, "prefix_capacity must be >= 0");
@@ -175,7 +176,8 @@ int set_up(wick_hip_batch *b) {
     b->lim.cus = prop.multiProcessorCount;
     b->max_items = wick::batch_max_items(b->lim);
     b->state_rows = wick::batch_max_state_rows(b->lim);
-    if (b->max_items * c.kv_heads > INT_MAX / 2 || b->state_rows > INT_MAX / 2)
+    // a launch holds 2^32 threads, and state rows are 32-bit numbers
+    if (b->max_items * c.kv_heads > (1 << 23) || b->state_rows > INT_MAX / 2)
         return set_error(WICK_HIP_EINVAL, "max_tokens %d is too large", c.max_tokens);
     b->items_at = sizeof(wick::BatchHeader) + (size_t)c.max_tokens * sizeof(wick::BatchToken);
     b->items_at = (b->items_at + 63) / 64 * 64;

@@ -24,7 +24,9 @@ namespace wick {
 constexpr int kBatchRows = 16;   // rows of a narrow item
 constexpr int kBatchWide = 128;  // rows of a wide item: 4 waves x 32
 constexpr int kBatchStep = 128;  // keys a narrow item takes at a time: 4 waves x 32
-constexpr int kBatchFew = 48;    // rows up to which narrow items share them
+// Rows up to which narrow items share them: 64 rows (32/4 heads of 64, prefix of 16000) 20.8 us, as
+// one wide item 24.1; 96 rows 30.3, as a wide one 26.9.
+constexpr int kBatchFew = 64;
 
 // One workgroup's work (device layout).
 struct BatchItem {
@@ -92,13 +94,20 @@ struct BatchPlan {
     int64_t state_rows = 0;
 };
 
-constexpr double kPlanItem = 2.0;       // an item's cost besides its keys'
-constexpr double kPlanJoin = 18.0;      // what leaving states and joining them costs a step
-constexpr double kPlanLone = 1.3;       // a tile's cost where a unit has one wide item, not two
-constexpr double kPlanLeastWide = 4.0;  // least cost of a range of keys
-constexpr double kPlanLeastNarrow = 1.0;
-constexpr double kPlanAlone = 3.0;      // up to which ranges are not cut to save the second launch
-constexpr double kPlanWideItems = 2.0;  // wide items to cut for each compute unit (narrow ones: one)
+// The constants of the plan, in tiles of 32 keys by a wide item (about 2 us at head_dim 128).
+constexpr double kPlanItem = 2.0;  // an item's cost besides its keys'
+// What leaving states and joining them costs a step, and what a tile of a lone wide item on a
+// unit takes against one of two.  16 prompts of 13..161 tokens behind a prefix of 1500 (16/8 heads
+// of 128): split 98 us, whole 128; one prompt of 512: 29.5 and 43.8; six prompts of 697..2047
+// (32/8 heads, bf16): 158 whole, 174 split.
+constexpr double kPlanJoin = 18.0, kPlanLone = 1.3;
+constexpr double kPlanLeastWide = 4.0, kPlanLeastNarrow = 1.0;  // least cost of a range of keys
+// Ranges up to which small sequences are not cut, to save the second launch: four tokens behind a
+// prefix of 100 (9/3 heads of 64) 6.8 us, cut 9.0; of 200 8.2 and 9.2; of 300 9.5 and 9.3.
+constexpr double kPlanAlone = 1.6;
+// Wide items to cut for each compute unit (narrow ones: one): 64 tokens over a prefix of 32768
+// (32/8 heads of 128, bf16) 126 us with two, 136 with 1.5, 142 with 2.5.
+constexpr double kPlanWideItems = 2.0;
 
 // Cost of a block of `rows` rows against `keys` keys, in tiles of a wave: a wide item's waves
 // all take every 32 keys, a narrow one's every fourth; and what an item costs besides.
@@ -116,11 +125,14 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
     auto rows_of = [&](int s) { return (int64_t)t[s] * c.group; };
     auto chunks = [](int64_t keys, int64_t len) { return (keys + len - 1) / len; };
 
-    // Wide blocks where, cut as finely as they may be, they give every compute unit an
-    // item; narrow ones in smaller steps, which are eight times as many.
-    int64_t most_wide = 0, small_rows = 0;
+    // Narrow blocks for a step that would leave units idle with wide ones, cut as finely as
+    // they may be, if one round of narrow ones holds it: 16 tokens over a prefix of 4001 (14/2
+    // heads of 64) 12.6 us, 15.2 with wide blocks; one prompt of 512 (16/8 of 128) 25.1 and 29.5; of
+    // 1000 (32/8 of 128) 98.7 and 80.8; eight of 50..100 (32/4 of 64) 14.2 and 10.9.
+    int64_t most_wide = 0, least_narrow = 0, small_rows = 0;
     for (int s = 0; s < c.sequences; s++) {
         const int64_t rows = rows_of(s), keys = (int64_t)start[s] + t[s];
+        least_narrow += chunks(rows, kBatchRows);
         if (rows > kBatchFew)
             most_wide += chunks(rows, kBatchWide) * chunks(prefix + keys, (int64_t)(32 * kPlanLeastWide));
         else
@@ -128,7 +140,7 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
     }
     if (small_rows > kBatchFew)
         most_wide += chunks(small_rows, kBatchWide) * chunks(prefix, (int64_t)(32 * kPlanLeastWide));
-    const bool wides = most_wide * c.kv_heads >= c.cus;
+    const bool wides = std::max(most_wide, least_narrow) * c.kv_heads >= 2 * c.cus;
     auto block_of = [&](int64_t rows) { return wides && rows > kBatchFew ? kBatchWide : kBatchRows; };
     auto blocks = [&](int64_t rows) { return chunks(rows, block_of(rows)); };
     auto big = [&](int s) { return block_of(rows_of(s)) == kBatchWide; };

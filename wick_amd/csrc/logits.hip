@@ -55,8 +55,8 @@ __global__ __launch_bounds__(kT) void logits_kernel(LogitArgs a) {
         if (mask && i < a.vocab) allowed[u] = mask[i >> 5] >> (i & 31);
     }
 
-    int n = r.tokens ? min(max(r.n_tokens[row], 0), r.tokens_stride) : 0;
-    const int prompt = n && r.n_prompt ? r.n_prompt[row] : 0;
+    const uint32_t n = r.tokens ? min(max(r.n_tokens[row], 0), r.tokens_stride) : 0;
+    const uint32_t prompt = n && r.n_prompt ? max(r.n_prompt[row], 0) : 0;
     int b0 = 0, b1 = 0;
     if (r.bias) {
         b0 = min(max(r.bias_start[row], 0), r.n_bias);
@@ -68,15 +68,15 @@ __global__ __launch_bounds__(kT) void logits_kernel(LogitArgs a) {
         for (int u = 0; u < U; u++) mine[u * kT] = u4{0, 0, 0, 0};
         __syncthreads();
         const uint32_t *tokens = r.tokens + (size_t)row * r.tokens_stride;
-        auto seen = [&](int i, uint32_t id) {
+        auto seen = [&](uint32_t i, uint32_t id) {
             const uint32_t at = id - (uint32_t)s0;
             if (at < (uint32_t)SLAB) {
                 atomicOr(&note[at], kSeen);
                 if (i >= prompt) atomicAdd(&note[at], 1u);
             }
         };
-        const int n4 = n & ~3;
-        for (int i = 4 * tid; i < n4; i += 4 * kT) {
+        const uint32_t n4 = n & ~3u;  // unsigned: a step past 2^31 tokens does not overflow
+        for (uint32_t i = 4 * tid; i < n4; i += 4 * kT) {
             const u4u id = *reinterpret_cast<const u4u *>(tokens + i);
 #pragma unroll
             for (int j = 0; j < 4; j++) seen(i + j, id[j]);
@@ -102,9 +102,9 @@ __global__ __launch_bounds__(kT) void logits_kernel(LogitArgs a) {
 #pragma unroll
         for (int u = 0; u < U; u++) mine[u * kT] = u4{0, 0, 0, 0};
         __syncthreads();
-        for (int i = b0 + tid; i < b1; i += kT) {
+        for (uint32_t i = b0 + tid; i < (uint32_t)b1; i += kT) {
             const uint32_t at = r.bias_ids[i] - (uint32_t)s0;
-            if (at < (uint32_t)SLAB) atomicMax(&note[at], (uint32_t)(i - b0) + 1);
+            if (at < (uint32_t)SLAB) atomicMax(&note[at], i - b0 + 1);
         }
         __syncthreads();
 #pragma unroll

@@ -14,6 +14,7 @@ extern "C" int wick_hip_logits_adjust_device(const wick_hip_logit_rules *rules, 
     if (!rules || !logits || !out) return set_error(WICK_HIP_EINVAL, "null argument");
     const wick_hip_logit_rules &r = *rules;
     if (rows < 0 || vocab < 1) return set_error(WICK_HIP_EINVAL, "rows must be >= 0 and vocab >= 1 (got %d, %d)", rows, vocab);
+    if (vocab > (1 << 30)) return set_error(WICK_HIP_EINVAL, "vocab must be at most 2^30 (got %d)", vocab);
     if (stride < vocab || out_stride < vocab)
         return set_error(WICK_HIP_EINVAL, "strides %d and %d must be at least vocab %d", stride, out_stride, vocab);
     if (r.tokens && !r.n_tokens) return set_error(WICK_HIP_EINVAL, "tokens without n_tokens");

@@ -1,5 +1,5 @@
 """ctypes wrapper of include/wick_hip_logits.h: penalties, biases and grammar masks on a
-batch's logits, the step of wick's sampler at /root/reference/src/sampler.rs:75-83 and
+batch's logits, the step of wick's sampler at src/sampler.rs:75-83 and
 what serving programs put next to it.
 """
 import ctypes
