@@ -278,6 +278,22 @@ def test_values_without_parts():
     assert bool(((got.double() - want).abs() <= tol).all())
 
 
+SCALES = [(1e20, 1e-20, 1e-30), (1e-18, 1e18, 1e30), (1.0, 1.0, 1e-20)]
+
+
+@pytest.mark.parametrize("q_by,k_by,v_by", SCALES)
+@pytest.mark.parametrize("n", [1, 90])
+def test_values_of_any_scale(q_by, k_by, v_by, n):
+    """Queries, keys and values far from 1, narrow items and wide: as exact as near it."""
+    c = Case(8, 2, 64, [40, 0], [n, n], 600, seed=13 + n)
+    c.q *= q_by
+    for x in [c.pk] + c.k:
+        x *= k_by
+    for x in [c.pv] + c.v:
+        x *= v_by
+    c.fill().check()
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_load_prefix_and_the_cache_it_came_from(dtype):
     """A prompt in a DeviceKvCache becomes the prefix; one more token attends as the cache's own call."""

@@ -13,10 +13,10 @@
 // f32 products on the bf16 matrix cores.  x = x1 + x2 + x3, each part the bf16 nearest to
 // what the ones before it leave (8 + 8 + 8 significant bits: exact but for the last part's
 // rounding, 2^-27 of x), and x y = sum of x_i y_j.  A part of index i is at most 2^-9(i-1)
-// of x, so the six products with i + j <= 4 leave out less than 2^-26 of |x y| -- under
-// half the rounding of an f32 product -- and the sums are the matrix cores' f32 ones.  Six bf16
+// of x, so the six products with i + j <= 4 leave out about 2^-26 of |x y| -- half the
+// rounding of an f32 product -- and the sums are the matrix cores' f32 ones.  Six bf16
 // products cost 6/16 of the f32 matrix instructions'.  A bf16 cache is its own first part:
-// three products.  Infinities and values next to f32's largest have no such parts (inf - inf),
+// three products.  (Values under 2^-108 lose low parts to underflow.)  Infinities and values next to f32's largest have no such parts (inf - inf),
 // nor may a hidden key's NaN times a weight of 0 count: either leaves a NaN or an infinity in
 // its row's state, and a row with one is computed again, key by key in f32 (redo_row).
 //
@@ -28,6 +28,14 @@
 // rows of the instruction are the dimensions d = (D / 32) (l % 32) + b, b = 0.. for the
 // D / 32 instructions, so that a lane reads D / 32 adjacent values of a key, and a half
 // wave a whole key.
+//
+// Bound.  Wide items: the matrix cores, at the rate that the card's power leaves them (a large
+// bf16 product reaches 1.16 PFLOP/s here, this instruction alone with random operands
+// 1.75).  Six prompts of 697..2047 tokens (32/8 heads of 128) take 0.39 to 0.41 ms: 76.9 GFLOP, six
+// times that in parts, 1.2 PFLOP/s; on a bf16 cache 53 GFLOP, three times, 0.16 ms, 1.0 PFLOP/s, where
+// the weights' vector instructions are the next limit.  A tile of 32 keys (head_dim 128, f32) takes
+// 4.06 us where a unit has two wide items and 2.7 where it has one, against 1.7 of products.  Narrow items:
+// the latency of a step's loads, then the split of its values; HBM where there are many.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
@@ -191,9 +199,12 @@ struct Shape {
     static constexpr int NB = D >= 32 ? D / 32 : 1;  // 32-dimension blocks of O
     static constexpr int KP = sizeof(T) == 4 ? 3 : 1;
     // a wide item's tile: 64 keys, or 32 where the parts of 64 would not leave room for two
-    // workgroups on a CU
+    // workgroups on a CU (one of them 437 us for the six prompts, two 403; tiles of 32 keys in
+    // all cases, a tile's values weighted next to the next tile's weights: eight prompts of 39..701
+    // (14/2 heads of 64) 39.1 us, as it is 36.0)
     static constexpr int KT = D == 128 && KP == 3 ? 32 : 64;
-    // q's third parts lie in LDS where all of them would not leave the registers for two
+    // q's third parts lie in LDS where all of them would not leave the registers for two (spilled,
+    // the six prompts took 614 us)
     static constexpr int QP = D == 128 ? 2 : 3;
     static constexpr int KF = KT / 32 * KS, VF = KT / 16 * NB;  // operands of a tile: K's, V's
     // a narrow item's, with 16x16x32 instructions
@@ -429,6 +440,7 @@ struct Few {
     using S = Shape<D, T>;
     static constexpr int KS = S::KS16, NB = S::NB16;
     // a step's keys and values are requested a step ahead where there are registers for both
+    // (else its values with its own scores, the next step's keys after them)
     static constexpr int AHEAD = D * sizeof(T) <= 256 ? 2 : 1;
     Parts<3> q[KS];
     f32x4 o[NB];
@@ -796,7 +808,10 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
 
 // W waves join one row's states: with the largest m, weights 2^(m_i - m), att = sum w O /
 // sum w l.  D / 4 lanes read a state, 8 states in flight each; their running sums are
-// joined last, always in the same order.
+// joined last, always in the same order.  Bound by the states' reads and its own launch: 1024 rows of
+// 28 states of 128 dimensions 7.6 us (one state after the other, as the first version read them, 19).
+// Four waves where one would need several rounds of its 8: there 72.5 us a step against 74.4 with
+// one, and with one for 23 thousand rows of 4 states (16 prompts behind a prefix) 98 against 119.
 template <int D, int W>
 __global__ __launch_bounds__(256) void batch_merge_kernel(BatchArgs a) {
     constexpr int L = D / 4, G = 64 * W / L, B = 8;  // lanes of a state, states at once, and on their way
@@ -962,7 +977,7 @@ struct MergeLaunch {
     hipStream_t s;
     template <int D, class T>
     hipError_t operator()() {
-        if (a.max_states > 256 / D * 8)
+        if (a.max_states > 256 / D * 8)  // one wave's round
             batch_merge_kernel<D, 4><<<(int)std::min<long long>(1 << 20, rows), 256, 0, s>>>(a);
         else
             batch_merge_kernel<D, 1><<<(int)std::min<long long>(1 << 20, (rows + 3) / 4), 256, 0, s>>>(a);

@@ -2,10 +2,12 @@
 //
 // A workgroup has one row's ids [s0, s0 + SLAB).  It requests its logits and mask words,
 // counts the row's tokens that fall into its slab in LDS (integer adds: any order gives
-// the same counts), notes each id's last bias there, then writes its part of the row.  A
-// row's tokens are read once per slab, from the L2.
+// the same counts) and applies the penalties, notes each id's last bias there and adds
+// them, then writes its part of the row.  A row's tokens are read once per slab, from the L2.
 //
-// Bound: HBM, 8 bytes a logit and a mask bit.
+// Bound: HBM, 8 bytes a logit and a mask bit: 64 rows of 128256 with 1500 tokens each 14.2 us, 4.7 TB/s
+// (a copy of as many bytes 10.1); one row of 49152 is the launch (3 us on the GPU).  One LDS word an
+// id, used for the counts and then for the biases: with a word for each the 64 rows took 18.1.
 #include <hip/hip_runtime.h>
 
 #include "logits_kernels.h"
