@@ -16,9 +16,10 @@
 // of x, so the six products with i + j <= 4 leave out about 2^-26 of |x y| -- half the
 // rounding of an f32 product -- and the sums are the matrix cores' f32 ones.  Six bf16
 // products cost 6/16 of the f32 matrix instructions'.  A bf16 cache is its own first part:
-// three products.  (Values under 2^-108 lose low parts to underflow.)  Infinities and values next to f32's largest have no such parts (inf - inf),
-// nor may a hidden key's NaN times a weight of 0 count: either leaves a NaN or an infinity in
-// its row's state, and a row with one is computed again, key by key in f32 (redo_row).
+// three products.  (Values under 2^-108 lose low parts to underflow.)  Infinities and values
+// next to f32's largest have no such parts (inf - inf), nor may a hidden key's NaN times a
+// weight of 0 count: either leaves a NaN or an infinity in its row's state, and a row with one
+// is computed again, key by key in f32 (redo_row).
 //
 // Layouts.  The 32x32x16 instruction gives lane l of a wave row (or column) l % 32 and, of the
 // 16 contracted indices, the 8 numbered 8 (l / 32)...  S^T leaves in lane l, for row l % 32, the keys
@@ -439,13 +440,10 @@ template <int D, class T>
 struct Few {
     using S = Shape<D, T>;
     static constexpr int KS = S::KS16, NB = S::NB16;
-    // a step's keys and values are requested a step ahead where there are registers for both
-    // (else its values with its own scores, the next step's keys after them)
-    static constexpr int AHEAD = D * sizeof(T) <= 256 ? 2 : 1;
     Parts<3> q[KS];
     f32x4 o[NB];
     float m, l;
-    T k[AHEAD][2][KS][8], v[AHEAD][8][NB];
+    T k[2][KS][8], v[8][NB];
 
     __device__ __forceinline__ void begin(const float *src, float scale, int quad) {
 #pragma unroll
@@ -463,31 +461,31 @@ struct Few {
     }
 
     // of n keys left at p
-    __device__ __forceinline__ void load_k(int to, const T *p, int n, int col, int quad) {
+    __device__ __forceinline__ void load_k(const T *p, int n, int col, int quad) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const unsigned at = min(16 * u + col, n - 1) * D + 8 * (D >= 32 ? quad : quad & 1);
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) load_n<8>(p + 32 * ks + at, k[to][u][ks]);
+            for (int ks = 0; ks < KS; ks++) load_n<8>(p + 32 * ks + at, k[u][ks]);
         }
     }
-    __device__ __forceinline__ void load_v(int to, const T *p, int n, int col, int quad) {
+    __device__ __forceinline__ void load_v(const T *p, int n, int col, int quad) {
 #pragma unroll
         for (int j = 0; j < 8; j++)
-            load_n<NB>(p + (unsigned)(min(16 * (j / 4) + 4 * quad + j % 4, n - 1) * D + NB * col), v[to][j]);
+            load_n<NB>(p + (unsigned)(min(16 * (j / 4) + 4 * quad + j % 4, n - 1) * D + NB * col), v[j]);
     }
 
-    __device__ __forceinline__ void scores(int at, f32x4 (&s)[2]) const {
+    __device__ __forceinline__ void scores(f32x4 (&s)[2]) const {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             s[u] = f32x4{};
 #pragma unroll
-            for (int ks = 0; ks < KS; ks++) s[u] = product(parts8(k[at][u][ks]), q[ks], s[u]);  // 16 dimensions: q's rest is 0
+            for (int ks = 0; ks < KS; ks++) s[u] = product(parts8(k[u][ks]), q[ks], s[u]);  // 16 dimensions: q's rest is 0
         }
     }
 
     // keys past `left` of the 32 are hidden
-    __device__ __forceinline__ void values(int at, f32x4 (&s)[2], bool mask, int left) {
+    __device__ __forceinline__ void values(f32x4 (&s)[2], bool mask, int left) {
         if (mask) {
 #pragma unroll
             for (int i = 0; i < 8; i++) s[i / 4][i % 4] = 16 * (i / 4) + i % 4 > left ? -INFINITY : s[i / 4][i % 4];
@@ -514,7 +512,7 @@ struct Few {
         for (int b = 0; b < NB; b++) {
             T y[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = v[at][j][b];
+            for (int j = 0; j < 8; j++) y[j] = v[j][b];
             o[b] = product(parts8(y), w, o[b]);
         }
     }
@@ -644,7 +642,6 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
                             for (int j = g * 4 / NB; j < (g + 1) * 4 / NB; j++) st.weight2(s[sub], w8[1], 1, 2 * j);
 #pragma unroll
                         for (int i = g * UNITS / G; i < (g + 1) * UNITS / G; i++) sk.store(sub * UNITS + i, kat, wave);
-
                         x = y;
                     }
                 }
@@ -719,40 +716,25 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
             const int tiles = np + max(0, (it.o1 - it.o0 - 32 * wave + 127) / 128);
             auto first_key = [&](int t) { return 32 * wave + (t < np ? it.p0 + 128 * t : it.o0 + 128 * (t - np)); };
             Few<D, T> st;
-            constexpr int AHEAD = Few<D, T>::AHEAD;
-            // past the last tile the last one again
-            auto load_k = [&](int to, int t) {
-                const int u = min(t, tiles - 1), key = first_key(u);
-                st.load_k(to, (u < np ? pk : ok) + (size_t)key * D, (u < np ? it.p1 : it.o1) - key, c, quad);
+            // a step's values are requested before its scores are summed, the next step's keys before
+            // its weights are taken.  Both a whole step ahead, where there are registers for it, took
+            // 12.9 us against 13.4 for 16 tokens over a prefix of 4001, but 9.05 against 8.6 for 4
+            // over 1025 and 4.95 against 4.7 for three short prompts.
+            auto load_k = [&](int t) {
+                const int key = first_key(t);
+                st.load_k((t < np ? pk : ok) + (size_t)key * D, (t < np ? it.p1 : it.o1) - key, c, quad);
             };
-            auto load_v = [&](int to, int t) {
-                const int u = min(t, tiles - 1), key = first_key(u);
-                st.load_v(to, (u < np ? pv : ov) + (size_t)key * D, (u < np ? it.p1 : it.o1) - key, c, quad);
-            };
-            if (tiles > 0) {
-                load_k(0, 0);
-                if (AHEAD == 2) load_v(0, 0);
-            }
+            if (tiles > 0) load_k(0);
             st.begin(a.q + row_at(r), a.scale, quad);
-            for (int t0 = 0; t0 < tiles; t0 += AHEAD) {
-#pragma unroll
-                for (int x = 0; x < AHEAD; x++) {
-                    const int t = t0 + x;
-                    if (x > 0 && t >= tiles) break;
-                    if (AHEAD == 2) {
-                        load_k(1 - x, t + 1);
-                        load_v(1 - x, t + 1);
-                    } else {
-                        load_v(0, t);
-                    }
-                    f32x4 s[2];
-                    st.scores(x, s);
-                    if (AHEAD == 1) load_k(0, t + 1);
-                    const bool o = t >= np;
-                    const int key0 = first_key(t), end = o ? it.o1 : it.p1;
-                    st.values(x, s, key0 + 32 > end || (o && key0 + 31 > first_last),
-                              (o ? min(last, end - 1) : end - 1) - key0 - 4 * quad);
-                }
+            for (int t = 0; t < tiles; t++) {
+                const bool o = t >= np;
+                const int key0 = first_key(t), end = o ? it.o1 : it.p1;
+                st.load_v((o ? ov : pv) + (size_t)key0 * D, end - key0, c, quad);
+                f32x4 s[2];
+                st.scores(s);
+                if (t + 1 < tiles) load_k(t + 1);
+                st.values(s, key0 + 32 > end || (o && key0 + 31 > first_last),
+                          (o ? min(last, end - 1) : end - 1) - key0 - 4 * quad);
             }
             const float l = rows_sum(st.l);
             // join the waves' states: O by row through LDS
