@@ -462,6 +462,41 @@ def test_graph_follows_the_plan(dtype, prefix):
     assert np.array_equal(before[0], after[0]) and np.array_equal(before[1], after[1])
 
 
+def test_shapes_are_known_again():
+    """A step of other tokens in between leaves a shape's number and its graphs; past 32 others a new number."""
+    c = Case(8, 2, 64, [40, 90, 7], [1, 1, 1], 150, seed=31).fill()
+    want = c.check()
+    n, stream = c.b.shape(), torch.cuda.Stream()
+    q, att = c.q.clone(), torch.empty_like(want)
+    torch.cuda.synchronize()
+    c.b.set_stream(stream.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        c.b.attention_device(c.layer, q.data_ptr(), att.data_ptr())
+
+    def replay():
+        c.b.plan(c.start, c.t, c.prefix)
+        with torch.cuda.stream(stream):
+            att.zero_()
+            graph.replay()
+        torch.cuda.synchronize()
+
+    for _ in range(3):
+        c.b.plan([0, 0, 0], [30, 0, 5], c.prefix)
+        assert c.b.shape() != n
+        replay()
+        assert c.b.shape() == n and torch.equal(att, want)
+    for i in range(31):
+        c.b.plan([0, 0, 0], [0, i + 2, 1], c.prefix)
+    replay()
+    assert c.b.shape() == n and torch.equal(att, want)
+    for i in range(32):
+        c.b.plan([0, 0, 0], [0, 2, i + 2 if i != 1 else 0], c.prefix)
+    replay()
+    assert c.b.shape() not in (0, n) and bool(torch.isnan(att).all())
+    assert torch.equal(c.run(), want)
+
+
 def test_offsets_past_32_bits():
     """The second sequence's and the second kv head's positions lie past 2^32 bytes and 2^31 values."""
     heads, kvh, d, cap = 4, 2, 128, 9_000_000

@@ -10,10 +10,12 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstring>
 #include <new>
+#include <utility>
 #include <vector>
 
 #include "attn_kernels.h"
@@ -37,7 +39,14 @@ struct wick_hip_batch {
     wick::BatchHeader head{};
     bool planned = false;
     int shape = 0;  // of the last plan
-    std::vector<int> counts;  // t of the shape
+    // the last plans' shapes, the newest at the end: a step of prompts between steps of answers
+    // leaves the answers' number, and the graphs captured under it, as they were
+    struct Shape {
+        std::vector<int> t;
+        int number;
+    };
+    std::vector<Shape> shapes;
+    int numbers = 0;  // given so far; none is given twice
     // staging of the host-array calls
     float *stage = nullptr;
     size_t stage_floats = 0;
@@ -57,6 +66,8 @@ struct wick_hip_batch {
 namespace {
 
 using wick::set_error;
+
+constexpr size_t kShapes = 32;  // plans whose shapes are known again
 
 int hip_fail(hipError_t e, const char *what) {
     return set_error(e == hipErrorOutOfMemory ? WICK_HIP_ENOMEM : WICK_HIP_EHIP, "%s: %s", what, hipGetErrorString(e));
@@ -182,7 +193,7 @@ int set_up(wick_hip_batch *b) {
     b->items_at = sizeof(wick::BatchHeader) + (size_t)c.max_tokens * sizeof(wick::BatchToken);
     b->items_at = (b->items_at + 63) / 64 * 64;
     b->plan_bytes = b->items_at + (size_t)b->max_items * sizeof(wick::BatchItem);
-    b->counts.assign(c.sequences, -1);
+    b->shapes.reserve(kShapes);
     HIP_TRY(hipStreamCreateWithFlags(&b->own_stream, hipStreamNonBlocking));
     b->stream = b->own_stream;
     HIP_TRY(hipEventCreateWithFlags(&b->moved, hipEventDisableTiming));
@@ -335,10 +346,17 @@ int wick_hip_batch_plan(wick_hip_batch *b, const int *start, const int *t, int p
         const int slot = b->plan_slot;
         HIP_TRY(hipEventSynchronize(b->plan_sent[slot]));
         // captured calls depend on the tokens of every sequence, and on nothing else of a plan
-        const bool same = std::memcmp(b->counts.data(), t, c.sequences * sizeof(int)) == 0;
-        if (!same) b->shape++;
-        p.head.shape = b->shape;
-        std::memcpy(b->counts.data(), t, c.sequences * sizeof(int));
+        auto known = std::find_if(b->shapes.begin(), b->shapes.end(), [&](const wick_hip_batch::Shape &x) {
+            return std::memcmp(x.t.data(), t, c.sequences * sizeof(int)) == 0;
+        });
+        if (known == b->shapes.end()) {
+            wick_hip_batch::Shape x{std::vector<int>(t, t + c.sequences), ++b->numbers};
+            if (b->shapes.size() == kShapes) b->shapes.erase(b->shapes.begin());
+            b->shapes.push_back(std::move(x));
+        } else {
+            std::rotate(known, known + 1, b->shapes.end());
+        }
+        b->shape = p.head.shape = b->shapes.back().number;
         char *h = b->plan_host[slot];
         const size_t tokens = p.tokens.size() * sizeof(wick::BatchToken), items = p.items.size() * sizeof(wick::BatchItem);
         std::memcpy(h, &p.head, sizeof p.head);
