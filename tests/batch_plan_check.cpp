@@ -103,6 +103,7 @@ int main() {
         c.capacity = pick(1, 300);
         c.prefix_capacity = k % 3 ? pick(0, 900) : 0;
         c.cus = k % 4 == 0 ? 16 : k % 4 == 1 ? 256 : k % 4 == 2 ? 1 : 64;
+        c.few = batch_few(k / 4 % 2);
         const bool single = k % 5 == 0;
         std::vector<int> start(c.sequences), t(c.sequences);
         int total = 0;

@@ -185,6 +185,7 @@ int set_up(wick_hip_batch *b) {
     b->lim.prefix_capacity = c.prefix_capacity;
     b->lim.max_tokens = c.max_tokens;
     b->lim.cus = prop.multiProcessorCount;
+    b->lim.few = wick::batch_few(c.type == WICK_HIP_BATCH_BF16);
     b->max_items = wick::batch_max_items(b->lim);
     b->state_rows = wick::batch_max_state_rows(b->lim);
     // a launch holds 2^32 threads, and state rows are 32-bit numbers

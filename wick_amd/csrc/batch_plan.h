@@ -24,9 +24,14 @@ namespace wick {
 constexpr int kBatchRows = 16;   // rows of a narrow item
 constexpr int kBatchWide = 128;  // rows of a wide item: 4 waves x 32
 constexpr int kBatchStep = 128;  // keys a narrow item takes at a time: 4 waves x 32
-// Rows up to which narrow items share them: 64 rows (32/4 heads of 64, prefix of 16000) 20.8 us, as
-// one wide item 24.1; 96 rows 30.3, as a wide one 26.9.
+// Rows up to which narrow items share them.  Of a sequence: 64 rows (32/4 heads of 64) over 16000
+// keys 20.8 us, as one wide item 24.1; 96 rows 30.3, as a wide one 26.9.
 constexpr int kBatchFew = 64;
+// Of several sequences against the prefix: narrow items each split f32 keys into parts again.  48 rows
+// (32/8 heads of 128) over a prefix of 32768 103 us, as a wide item 81; 33 to 64 rows over 8000 to
+// 24000 take from 3% less to 17% more as narrow ones.  A bf16 cache's keys need no split: 64 rows over
+// 16000 30.4 us, as a wide item 35.5.
+inline int batch_few(bool bf16) { return bf16 ? 64 : 32; }
 
 // One workgroup's work (device layout).
 struct BatchItem {
@@ -69,6 +74,7 @@ static_assert(sizeof(BatchHeader) == 64, "");
 struct BatchLimits {
     int group, kv_heads, sequences, capacity, prefix_capacity, max_tokens;
     int cus;  // the GPU's compute units
+    int few;  // batch_few() of the cache's type
 };
 
 // Most items and state rows (per kv head) of any plan.  A big sequence is split only where
@@ -138,10 +144,11 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
         else
             small_rows += rows;
     }
-    if (small_rows > kBatchFew)
+    if (small_rows > c.few)
         most_wide += chunks(small_rows, kBatchWide) * chunks(prefix, (int64_t)(32 * kPlanLeastWide));
     const bool wides = std::max(most_wide, least_narrow) * c.kv_heads >= 2 * c.cus;
     auto block_of = [&](int64_t rows) { return wides && rows > kBatchFew ? kBatchWide : kBatchRows; };
+    auto shared_of = [&](int64_t rows) { return wides && rows > c.few ? kBatchWide : kBatchRows; };  // against the prefix
     auto blocks = [&](int64_t rows) { return chunks(rows, block_of(rows)); };
     auto big = [&](int s) { return block_of(rows_of(s)) == kBatchWide; };
 
@@ -170,7 +177,7 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
         base += 2 * chunks(rows, kBatchRows) + 1;
     }
     if (prefix && small_rows)
-        sum += blocks(small_rows) * (batch_cost(block_of(small_rows), prefix) + kPlanItem);
+        sum += chunks(small_rows, shared_of(small_rows)) * (batch_cost(shared_of(small_rows), prefix) + kPlanItem);
     const double share = sum * c.kv_heads / c.cus, target = wides ? share / kPlanWideItems : share;
     p.head.most_items = (int)std::min<int64_t>(batch_max_items(c), 2 * c.cus / c.kv_heads + 1 + 2 * base);
     const bool alone = alone_most <= kPlanAlone && alone_sum * c.kv_heads <= kPlanAlone * c.cus;
@@ -178,11 +185,11 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
         return big(s) ? kPlanLone * batch_cost(kBatchWide, (int64_t)prefix + start[s] + t[s]) <= share + kPlanJoin : alone;
     };
 
-    // n even ranges over the keys of a block of `rows` rows, each near the target, in steps
-    auto range = [&](int64_t rows, int keys) {
-        const bool wide = block_of(rows) == kBatchWide;
+    // n even ranges over the keys of a block, each near the target, in steps
+    auto range = [&](int block, int keys) {
+        const bool wide = block == kBatchWide;
         const double least = wide ? kPlanLeastWide : kPlanLeastNarrow;
-        const int n = std::max(1, (int)(batch_cost(block_of(rows), keys) / std::max(target, least) + 0.999));
+        const int n = std::max(1, (int)(batch_cost(block, keys) / std::max(target, least) + 0.999));
         const int part = (keys + n - 1) / n;
         const int step = wide ? 32 : kBatchStep;
         return (part + step - 1) / step * step;
@@ -195,7 +202,7 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
             for (int i = 0; i < t[s]; i++) split_token.push_back(token + i);
         }
     if (prefix && split_rows) {
-        const int part = range(split_rows, prefix), n = (int)chunks(prefix, part), step = block_of(split_rows);
+        const int step = shared_of(split_rows), part = range(step, prefix), n = (int)chunks(prefix, part);
         p.head.prefix_chunks = n;
         p.head.prefix_stride = (int)split_rows;
         for (int k = 0; k < n; k++) {
@@ -239,7 +246,7 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
         if (rows && whole(s)) {
             for (int r = 0; r < rows; r += step) block(r, 0, keys, -1, prefix);
         } else if (rows) {
-            const int part = range(rows, keys), n = (int)chunks(keys, part);
+            const int part = range(step, keys), n = (int)chunks(keys, part);
             const bool direct = n == 1 && !prefix;
             for (int i = 0; i < t[s] && !direct; i++) {
                 BatchToken &m = p.tokens[split];
