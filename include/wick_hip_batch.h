@@ -79,9 +79,10 @@ int wick_hip_batch_plan(wick_hip_batch *b, const int *start, const int *t, int p
 /* For callers that capture append and attention calls into a graph: the number of the
  * plan's launch shape.  Graphs captured under a plan replay under any later plan of the
  * same number (single tokens whose positions move on, for example), with that plan's
- * positions; the caller orders a replay on another stream with the handle's.  Plans with the
- * same t have the same number while it is among the last 32 that were planned.  Replayed under
- * a plan of another number graphs write NaN to every captured row of att, and append nothing. */
+ * positions, and within rounding of direct calls' results; the caller orders a replay on
+ * another stream with the handle's.  Plans with the same t have the same number while it is
+ * among the last 32 that were planned.  Replayed under a plan of another number graphs write
+ * NaN to every captured row of att, and append nothing. */
 int wick_hip_batch_shape(const wick_hip_batch *b);
 
 /* k and v of the planned tokens, device arrays [tokens][kv_heads*head_dim], 16-byte

@@ -788,12 +788,44 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
     }
 }
 
+// The running sums of a row's states c = first, first + G, ...: `B` of them on their way at a time.
+// base: state row 0 of the row's kv head, and the head in the group.
+template <int D, int G, int B>
+__device__ __forceinline__ void join_states(const BatchArgs &a, const BatchToken &t, size_t base, int prefix_chunks,
+                                            int stride, int first, int n, int d, float &m, float &l, f32x4 &acc) {
+    for (int c0 = first; c0 < n; c0 += B * G) {
+        f32x4 o[B];
+        float mm[B], ll[B], top = m;
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            const int c = min(c0 + b * G, n - 1);
+            const size_t at = base + (c < prefix_chunks ? t.prefix_state + (size_t)c * stride
+                                                        : t.own_state + (size_t)(c - prefix_chunks) * t.own_stride);
+            o[b] = *reinterpret_cast<const f32x4 *>(a.po + at * D + d);
+            mm[b] = a.pm[at];
+            ll[b] = a.pl[at];
+        }
+#pragma unroll
+        for (int b = 0; b < B; b++) top = fmaxf(top, mm[b]);
+        const float old = exp2f(m - top);
+        l *= old;
+        acc *= old;
+        m = top;
+#pragma unroll
+        for (int b = 0; b < B; b++)
+            if (c0 + b * G < n) {
+                const float f = exp2f(mm[b] - top);
+                l += f * ll[b];
+                acc += f * o[b];
+            }
+    }
+}
+
 // W waves join one row's states: with the largest m, weights 2^(m_i - m), att = sum w O /
 // sum w l.  D / 4 lanes read a state, 8 states in flight each; their running sums are
 // joined last, always in the same order.  Bound by the states' reads and its own launch: 1024 rows of
 // 28 states of 128 dimensions 7.6 us (one state after the other, as the first version read them, 19).
-// Four waves where one would need several rounds of its 8: there 72.5 us a step against 74.4 with
-// one, and with one for 23 thousand rows of 4 states (16 prompts behind a prefix) 98 against 119.
+// Four waves where one would need several rounds of its 8: there 72.5 us a step against 74.4 with one.
 template <int D, int W>
 __global__ __launch_bounds__(256) void batch_merge_kernel(BatchArgs a) {
     constexpr int L = D / 4, G = 64 * W / L, B = 8;  // lanes of a state, states at once, and on their way
@@ -812,32 +844,7 @@ __global__ __launch_bounds__(256) void batch_merge_kernel(BatchArgs a) {
         const int n = prefix_chunks + t.own_chunks;
         float m = kNoMax, l = 0.0f;
         f32x4 acc{};
-        for (int c0 = g; c0 < n; c0 += B * G) {
-            f32x4 o[B];
-            float mm[B], ll[B], top = m;
-#pragma unroll
-            for (int b = 0; b < B; b++) {
-                const int c = min(c0 + b * G, n - 1);
-                const size_t at = base + (c < prefix_chunks ? t.prefix_state + (size_t)c * stride
-                                                            : t.own_state + (size_t)(c - prefix_chunks) * t.own_stride);
-                o[b] = *reinterpret_cast<const f32x4 *>(a.po + at * D + d);
-                mm[b] = a.pm[at];
-                ll[b] = a.pl[at];
-            }
-#pragma unroll
-            for (int b = 0; b < B; b++) top = fmaxf(top, mm[b]);
-            const float old = exp2f(m - top);
-            l *= old;
-            acc *= old;
-            m = top;
-#pragma unroll
-            for (int b = 0; b < B; b++)
-                if (c0 + b * G < n) {
-                    const float f = exp2f(mm[b] - top);
-                    l += f * ll[b];
-                    acc += f * o[b];
-                }
-        }
+        join_states<D, G, B>(a, t, base, prefix_chunks, stride, g, n, d, m, l, acc);
         float top = m;
 #pragma unroll
         for (int x = L; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x, 64));
@@ -877,6 +884,26 @@ __global__ __launch_bounds__(256) void batch_merge_kernel(BatchArgs a) {
         f = 1.0f / l;
         if (lane < L && (W == 1 || wave == 0))
             *reinterpret_cast<f32x4 *>(a.att + ((size_t)t.merge * heads + head) * D + d) = acc * f;
+    }
+}
+
+// The same for few states: D / 4 lanes have a row, 4 states in flight, nothing to join across lanes.
+// 16 prompts of 12..161 tokens behind a prefix of 1500 (20 thousand rows) 102.4 us a step, 106.8
+// with a wave a row; 4 tokens over 300 (36 rows) 8.1 and 8.6; but 16 tokens of 14 states 14.5 and 13.4.
+template <int D>
+__global__ __launch_bounds__(256) void batch_merge_rows_kernel(BatchArgs a) {
+    constexpr int L = D / 4, R = 256 / L;  // lanes of a row, rows of a workgroup
+    const int d = 4 * (threadIdx.x % L), heads = a.group * a.kv_heads;
+    if (a.head->shape != a.shape) return;
+    const int work = a.head->merges * heads, prefix_chunks = a.head->prefix_chunks, stride = a.head->prefix_stride;
+    for (int w = blockIdx.x * R + threadIdx.x / L; w < work; w += gridDim.x * R) {
+        const int i = divide(w, heads, a.inv_heads), head = w - i * heads, kh = divide(head, a.group, a.inv_group);
+        const BatchToken t = a.tokens[i];
+        float m = kNoMax, l = 0.0f;
+        f32x4 acc{};
+        join_states<D, 1, 4>(a, t, (size_t)kh * a.state_rows + (head - kh * a.group), prefix_chunks, stride, 0,
+                             prefix_chunks + t.own_chunks, d, m, l, acc);
+        *reinterpret_cast<f32x4 *>(a.att + ((size_t)t.merge * heads + head) * D + d) = acc * (1.0f / l);
     }
 }
 
@@ -959,7 +986,9 @@ struct MergeLaunch {
     hipStream_t s;
     template <int D, class T>
     hipError_t operator()() {
-        if (a.max_states > 256 / D * 8)  // one wave's round
+        if (a.max_states <= 8)
+            batch_merge_rows_kernel<D><<<(int)std::min<long long>(1 << 20, (rows + 1024 / D - 1) / (1024 / D)), 256, 0, s>>>(a);
+        else if (a.max_states > 256 / D * 8)  // one wave's round
             batch_merge_kernel<D, 4><<<(int)std::min<long long>(1 << 20, rows), 256, 0, s>>>(a);
         else
             batch_merge_kernel<D, 1><<<(int)std::min<long long>(1 << 20, (rows + 3) / 4), 256, 0, s>>>(a);
