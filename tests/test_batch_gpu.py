@@ -157,6 +157,13 @@ def test_long_prefix_many_sequences(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("n", [4, 5, 8, 9, 13, 16, 17, 33])
+def test_rows_against_a_long_prefix(n, dtype):
+    """Single tokens of n sequences, 4 rows each: one to three narrow items or wide ones, some of their rows empty."""
+    Case(32, 8, 128, [(17 * s) % 50 for s in range(n)], [1] * n, 8300, dtype, seed=n).fill().check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("d", [16, 32, 64, 128])
 def test_many_states_of_a_row(d, dtype):
     """One token over a long context: its keys are dealt to over a hundred workgroups."""
