@@ -193,6 +193,9 @@ __device__ __forceinline__ float other_half(float v) {
     return __uint_as_float((threadIdx.x & 32) ? p[0] : p[1]);
 }
 
+// Whether the plan in memory is one that the call was made for (a replayed graph's may not be).
+__device__ __forceinline__ bool fits(const BatchArgs &a) { return a.head->shape == a.shape && a.head->items <= a.launched; }
+
 // What the kernel's shape fixes.
 template <int D, class T>
 struct Shape {
@@ -533,15 +536,13 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);  // the same in all lanes
     const int heads = a.group * a.kv_heads;
 
-    // the plan in memory does not fit the call (a replayed graph)
-    const int work = a.head->items * a.kv_heads;
-    if (a.head->shape != a.shape || work > (int)gridDim.x) {
+    if (!fits(a)) {
         const size_t n = (size_t)a.total * heads * D;
         for (size_t i = (size_t)blockIdx.x * 256 + tid; i < n; i += (size_t)gridDim.x * 256)
             a.att[i] = __builtin_nanf("");
         return;
     }
-    if ((int)blockIdx.x >= work) return;
+    if ((int)blockIdx.x >= a.head->items * a.kv_heads) return;
     {
         const int item = divide(blockIdx.x, a.kv_heads, a.inv_kv_heads), kh = blockIdx.x - item * a.kv_heads;
         const BatchItem it = a.items[item];
@@ -833,7 +834,7 @@ __global__ __launch_bounds__(256) void batch_merge_kernel(BatchArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = 4 * (lane % L);
     const int g = (W > 1 ? wave * (64 / L) : 0) + lane / L;
     const int heads = a.group * a.kv_heads;
-    if (a.head->shape != a.shape) return;
+    if (!fits(a)) return;
     const int work = a.head->merges * heads, prefix_chunks = a.head->prefix_chunks, stride = a.head->prefix_stride;
     constexpr int R = 4 / W;  // rows of a workgroup
     for (int w = blockIdx.x * R + (W > 1 ? 0 : wave); w < work; w += gridDim.x * R) {
@@ -894,7 +895,7 @@ template <int D>
 __global__ __launch_bounds__(256) void batch_merge_rows_kernel(BatchArgs a) {
     constexpr int L = D / 4, R = 256 / L;  // lanes of a row, rows of a workgroup
     const int d = 4 * (threadIdx.x % L), heads = a.group * a.kv_heads;
-    if (a.head->shape != a.shape) return;
+    if (!fits(a)) return;
     const int work = a.head->merges * heads, prefix_chunks = a.head->prefix_chunks, stride = a.head->prefix_stride;
     for (int w = blockIdx.x * R + threadIdx.x / L; w < work; w += gridDim.x * R) {
         const int i = divide(w, heads, a.inv_heads), head = w - i * heads, kh = divide(head, a.group, a.inv_group);

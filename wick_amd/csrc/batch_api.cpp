@@ -341,8 +341,8 @@ int wick_hip_batch_plan(wick_hip_batch *b, const int *start, const int *t, int p
     if (capturing(b->stream)) return set_error(WICK_HIP_EINVAL, "wick_hip_batch_plan on a stream that is being captured");
     try {
         wick::BatchPlan p = wick::batch_plan(b->lim, start, t, prefix);
-        if ((int64_t)p.items.size() > b->max_items || p.state_rows > b->state_rows)
-            return set_error(WICK_HIP_EHIP, "internal: the plan has %zu items and %lld state rows", p.items.size(),
+        if (p.head.items > b->max_items || p.head.items > p.head.most_items || p.state_rows > b->state_rows)
+            return set_error(WICK_HIP_EHIP, "internal: the plan has %d items and %lld state rows", p.head.items,
                              (long long)p.state_rows);
         const int slot = b->plan_slot;
         HIP_TRY(hipEventSynchronize(b->plan_sent[slot]));
@@ -438,6 +438,7 @@ int wick_hip_batch_attention_device(wick_hip_batch *b, int layer, const float *q
     // where this one has none
     const bool later = capturing(b->stream);
     const int items = later ? b->head.most_items : b->head.items;
+    a.launched = items;
     HIP_TRY(wick::launch_batch_attend(c.head_dim, c.type, a, items * c.kv_heads, b->stream));
     const int merges = later ? b->head.total : b->head.merges;
     if (merges) HIP_TRY(wick::launch_batch_merge(c.head_dim, a, merges, b->stream));

@@ -21,6 +21,7 @@ struct BatchArgs {
     int prefix_capacity, capacity, group, kv_heads;
     unsigned inv_group, inv_kv_heads, inv_heads;  // batch_inverse of group, kv_heads and their product
     int shape, total;  // of the plan at the call
+    int launched;      // items that the call has workgroups for
     int max_states;    // most states of a row in it
     float scale;       // log2(e) / sqrt(D)
 };

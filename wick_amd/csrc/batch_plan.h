@@ -77,11 +77,16 @@ struct BatchLimits {
     int few;  // batch_few() of the cache's type
 };
 
-// Most items and state rows (per kv head) of any plan.  A big sequence is split only where
-// its longest item costs more than 1 / kPlanLone of a unit's share, and its items cost half the
-// longest each or more, so that the split ones have at most 2.6 cus / kv_heads blocks together;
-// steps without wide blocks have fewer than cus / kv_heads of them; other sequences have up to
-// kBatchFew rows.  Ranges of a block are at most its cost over the target and one more.
+// Most items and state rows (per kv head) of any plan.  The cut prices every block in the shape it
+// is cut in, and a range costs the target or more, so the ranges of all blocks are at most their
+// costs over the target -- 2 cus / kv_heads together, or half of that without wide blocks -- and one
+// more a block.  Two more where a wide block's own keys end inside a range, which the average of
+// its rows' keys also prices half a range too low.  Blocks: a sequence of r rows has up to r / 16 + 1
+// of its own (wide ones an eighth of that), all split rows together up to r / 16 + 1 against the prefix.
+// A big sequence is split only where its longest item costs more than 1 / kPlanLone
+// of a unit's share, and its items cost half the longest each or more, so that the split
+// ones have at most 2.6 cus / kv_heads blocks together; steps without wide blocks have fewer
+// than 2 cus / kv_heads of them; other sequences have up to kBatchFew rows.
 inline int64_t batch_max_items(const BatchLimits &c) {
     const int64_t rows = (int64_t)c.max_tokens * c.group;
     return 2 * (rows / kBatchRows + std::min(c.sequences, c.max_tokens) + 1) + 2 * c.cus / c.kv_heads + 1;
@@ -176,14 +181,28 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
         }
         base += 2 * chunks(rows, kBatchRows) + 1;
     }
-    if (prefix && small_rows)
-        sum += chunks(small_rows, shared_of(small_rows)) * (batch_cost(shared_of(small_rows), prefix) + kPlanItem);
-    const double share = sum * c.kv_heads / c.cus, target = wides ? share / kPlanWideItems : share;
+    // the rows of the sequences that are not big, against the prefix in blocks of this shape
+    auto with_shared = [&](int block) {
+        return prefix && small_rows ? sum + chunks(small_rows, block) * (batch_cost(block, prefix) + kPlanItem) : sum;
+    };
+    const double share = with_shared(shared_of(small_rows)) * c.kv_heads / c.cus;
     p.head.most_items = (int)std::min<int64_t>(batch_max_items(c), 2 * c.cus / c.kv_heads + 1 + 2 * base);
     const bool alone = alone_most <= kPlanAlone && alone_sum * c.kv_heads <= kPlanAlone * c.cus;
     auto whole = [&](int s) {
         return big(s) ? kPlanLone * batch_cost(kBatchWide, (int64_t)prefix + start[s] + t[s]) <= share + kPlanJoin : alone;
     };
+
+    int64_t split_rows = 0;
+    std::vector<int> split_token;
+    for (int s = 0, token = 0; s < c.sequences; token += t[s++])
+        if (!whole(s)) {
+            split_rows += rows_of(s);
+            for (int i = 0; i < t[s]; i++) split_token.push_back(token + i);
+        }
+    // What a range should cost.  Split big sequences make the blocks of all split rows wide: there the
+    // other sequences' few rows add up to a wide block, not the narrow ones of a step of their own.
+    const double cost = with_shared(shared_of(alone ? small_rows : split_rows)) * c.kv_heads / c.cus;
+    const double target = wides ? cost / kPlanWideItems : cost;
 
     // n even ranges over the keys of a block, each near the target, in steps
     auto range = [&](int block, int keys) {
@@ -194,13 +213,6 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
         const int step = wide ? 32 : kBatchStep;
         return (part + step - 1) / step * step;
     };
-    int64_t split_rows = 0;
-    std::vector<int> split_token;
-    for (int s = 0, token = 0; s < c.sequences; token += t[s++])
-        if (!whole(s)) {
-            split_rows += rows_of(s);
-            for (int i = 0; i < t[s]; i++) split_token.push_back(token + i);
-        }
     if (prefix && split_rows) {
         const int step = shared_of(split_rows), part = range(step, prefix), n = (int)chunks(prefix, part);
         p.head.prefix_chunks = n;
