@@ -21,7 +21,8 @@
  * q and att are f32.  The caches hold f32 (WICK_HIP_BATCH_F32) or bfloat16
  * (WICK_HIP_BATCH_BF16: keys and values are rounded to nearest when they are written,
  * half the memory and half the bytes of a step); products of either are exact to f32
- * rounding (of values of 2^-108 and above), and every sum is f32.  Positions that a token does not see never reach
+ * rounding (of values of 2^-108 and above), and every sum is f32.  Scores times log2(e) that
+ * leave f32's range count as infinities.  Positions that a token does not see never reach
  * its result, whatever they hold (infinities and NaN included).
  *
  * Return codes, wick_hip_last_error() and the rules on handles as in wick_hip.h: calls on

@@ -54,8 +54,9 @@ typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 
-// A state without keys: finite, so that exp2(m - m) of two such is 1 and not NaN.
-constexpr float kNoMax = -3.0e38f;
+// The maximum of a state without keys: f32's lowest value, so that no finite score is below it, and
+// exp2(m - m) of two such is 1 and not NaN.
+constexpr float kNoMax = -3.40282347e38f;
 // The reference maximum is raised only when a score passes it by this (in log2 units):
 // weights then stay below 2^8, and the rescaling of O is rare.
 constexpr float kSlack = 8.0f;
@@ -676,7 +677,8 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
                 __syncthreads();
             }
             const float sum = st.l + other_half(st.l);
-            bool odd = !(fabsf(sum) < INFINITY);
+            // 0 though there are keys: their scores left f32 as sums of parts (or are -infinity)
+            bool odd = !(fabsf(sum) < INFINITY) || (sum == 0.0f && (it.p1 > it.p0 || last >= it.o0));
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -769,7 +771,7 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
 #pragma unroll
             for (int e = 0; e < E; e++) acc[e] += f * j.o[i][row][d0 + e];
         }
-        bool odd = !(fabsf(sum) < INFINITY);
+        bool odd = !(fabsf(sum) < INFINITY) || (sum == 0.0f && (it.p1 > it.p0 || last_of(row) >= it.o0));
 #pragma unroll
         for (int e = 0; e < E; e++) odd |= !(fabsf(acc[e]) < INFINITY);
         if (odd && row < it.nrows) j.redo[row] = 1;
