@@ -1,4 +1,5 @@
-"""The batch's attention at the ends of f32's range: scores next to its lowest value.
+"""The batch's attention at the ends of f32's range: scores next to its lowest value, values whose
+unweighted sums pass its largest.
 
 Tolerances as in test_batch_gpu; where all keys of a row are the same its weights are too, whatever
 their score, and the result is off by the sums' roundings alone: (0.75 n + 20) u sum_j w_j |v_j|.
@@ -11,6 +12,7 @@ import torch
 from test_batch_gpu import DEV, U, Case
 
 pytestmark = pytest.mark.gpu
+LARGEST = 3.4028234663852886e38  # of f32
 
 # heads, kv_heads, d, start, t, prefix: whole narrow items, whole wide ones, split ones of both kinds
 STEPS = [
@@ -67,3 +69,51 @@ def test_one_score_above_the_lowest(dtype):
     for rows, v in ((got[:90], c.v[0]), (got[90:], c.v[1])):
         v = v[2].to(c.dtype).float().view(1, 2, 1, 64)
         assert torch.equal(rows, v.expand_as(rows))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("step", STEPS)
+def test_values_whose_sum_has_no_room(step, dtype):
+    """Values up to f32's largest in every third dimension, ordinary ones in the others."""
+    c = Case(*step, dtype, seed=3)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    for x in [c.pv] + c.v:
+        big = (torch.rand(x[:, ::3].shape, generator=g, device=DEV) * 0.5 + 0.5) * 3.38e38
+        x[:, ::3] = torch.where(torch.rand(big.shape, generator=g, device=DEV) < 0.8, big, -big)
+    got = c.fill().run()
+    want, tol = c.want()
+    assert bool(torch.isfinite(got).all())
+    assert bool(((got.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("step", STEPS)
+def test_all_values_the_largest(step, dtype):
+    """Their mean is the largest value itself, and never an infinity."""
+    c = Case(*step, dtype, seed=5)
+    top = LARGEST if dtype == "f32" else torch.finfo(torch.bfloat16).max
+    for x in [c.pv] + c.v:
+        x.fill_(top)
+        x[:, 1::2] = -top
+    got = c.fill().run()
+    want, tol = c.want()
+    assert bool(torch.isfinite(got).all())
+    assert bool(((got.double() - want).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_an_infinite_value_stays_infinite(dtype):
+    """Beside values whose sum has no room: a seen infinity is the result's, a hidden one is not."""
+    c = Case(8, 2, 64, [0, 40], [60, 1], 3000, dtype, seed=6)
+    for x in [c.pv] + c.v:
+        x.fill_(3.0e38)
+    c.v[0][30, 5], c.v[0][31, 6] = math.inf, -math.inf
+    c.v[1][7, 9] = math.nan
+    got = c.fill().run().view(-1, 2, 4, 64)
+    odd = torch.zeros_like(got, dtype=torch.bool)
+    odd[30:60, 0, :, 5] = odd[31:60, 0, :, 6] = odd[60, 0, :, 9] = True
+    assert not bool(torch.isfinite(got[odd]).any())
+    rest = got[~odd].double()
+    # every value is the same: off by the sums' roundings over n <= 3060 keys
+    v = float(torch.tensor(3.0e38).to(c.dtype))
+    assert bool(((rest - v).abs() <= (0.75 * 3060 + 20) * U * v).all())

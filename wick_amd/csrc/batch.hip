@@ -17,9 +17,9 @@
 // rounding of an f32 product -- and the sums are the matrix cores' f32 ones.  Six bf16
 // products cost 6/16 of the f32 matrix instructions'.  A bf16 cache is its own first part:
 // three products.  (Values under 2^-108 lose low parts to underflow.)  Infinities and values
-// next to f32's largest have no such parts (inf - inf), nor may a hidden key's NaN times a
-// weight of 0 count: either leaves a NaN or an infinity in its row's state, and a row with one
-// is computed again, key by key in f32 (redo_row).
+// next to f32's largest have no such parts (inf - inf), large values' sums may overflow where
+// their mean does not, nor may a hidden key's NaN times a weight of 0 count: each leaves a NaN or
+// an infinity in its row's state, and a row with one is computed again, key by key in f32 (redo_row).
 //
 // Layouts.  The 32x32x16 instruction gives lane l of a wave row (or column) l % 32 and, of the
 // 16 contracted indices, the 8 numbered 8 (l / 32)...  S^T leaves in lane l, for row l % 32, the keys
@@ -301,19 +301,31 @@ struct StageV {
     }
 };
 
-// One row again in f32, key by key by one wave, over the item's keys that it sees: the
-// definition itself, for rows with a value that the parts have no room for.  Lane d has
-// the dimensions d, d + 64.
+// Sums of weights times values may pass f32's range where their mean does not.  2^-32 of them never
+// do: a row has less than 2^31 keys.  A row that needs it has its sums a second time at 2^-32,
+// which take the place of those that overflowed; a state with any such sum has all of them
+// at 2^-32 and says so by -l.
+constexpr float kLow = 0x1p-32f, kLargest = 3.40282347e38f;
+
+// low / l where sum overflowed and low did not: there the mean of finite values, which rounding may
+// bring past the largest.  All others are `mean`.
+__device__ __forceinline__ float mean_of(float sum, float mean, float low, float l) {
+    if (fabsf(sum) < INFINITY || !(fabsf(low) < INFINITY)) return mean;
+    return fminf(fmaxf(low / l, -kLargest), kLargest);
+}
+
+// One row again in f32, key by key by one wave, over the item's keys that it sees, for rows with a
+// value that the parts, or the sums, have no room for.  Lane d has the dimensions d, d + 64.
 template <int D, class T>
 __device__ __noinline__ void redo_row(const float *q, float scale, const T *pk, const T *pv, int p0, int p1, const T *k,
                                       const T *v, int o0, int o1, bool direct, float *dst, float *m_out, float *l_out) {
     const int lane = threadIdx.x & 63;
     constexpr int N = (D + 63) / 64;
-    float x[N], acc[N];
+    float x[N], acc[N], low[N];
 #pragma unroll
     for (int i = 0; i < N; i++) {
         x[i] = lane + 64 * i < D ? q[lane + 64 * i] * scale : 0.0f;
-        acc[i] = 0.0f;
+        acc[i] = low[i] = 0.0f;
     }
     float m = kNoMax, l = 0.0f;
     for (int part = 0; part < 2; part++) {
@@ -329,22 +341,36 @@ __device__ __noinline__ void redo_row(const float *q, float scale, const T *pk, 
                 const float f = exp2f(m - s);
                 l *= f;
 #pragma unroll
-                for (int i = 0; i < N; i++) acc[i] *= f;
+                for (int i = 0; i < N; i++) {
+                    acc[i] *= f;
+                    low[i] *= f;
+                }
                 m = s;
             }
             const float p = exp2f(s - m);
             l += p;
 #pragma unroll
             for (int i = 0; i < N; i++)
-                if (lane + 64 * i < D) acc[i] += p * (float)vv[(size_t)key * D + lane + 64 * i];
+                if (lane + 64 * i < D) {
+                    const float y = (float)vv[(size_t)key * D + lane + 64 * i];
+                    acc[i] += p * y;
+                    low[i] += p * kLow * y;
+                }
         }
     }
+    bool over = false;
+#pragma unroll
+    for (int i = 0; i < N; i++) over |= !(fabsf(acc[i]) < INFINITY) && fabsf(low[i]) < INFINITY;
+    const bool scaled = !direct && __any(over);
 #pragma unroll
     for (int i = 0; i < N; i++)
-        if (lane + 64 * i < D) dst[lane + 64 * i] = direct ? acc[i] / l : acc[i];
+        if (lane + 64 * i < D)
+            dst[lane + 64 * i] = direct    ? mean_of(acc[i], acc[i] / l, low[i], l * kLow)
+                                 : !scaled ? acc[i]
+                                           : fabsf(acc[i]) < INFINITY ? acc[i] * kLow : low[i];
     if (!direct && lane == 0) {
         *m_out = m;
-        *l_out = l;
+        *l_out = scaled ? -l : l;
     }
 }
 
@@ -791,8 +817,13 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
     }
 }
 
+// State c of a row.  base: state row 0 of the row's kv head, and the head in the group.
+__device__ __forceinline__ size_t state_of(const BatchToken &t, size_t base, int prefix_chunks, int stride, int c) {
+    return base + (c < prefix_chunks ? t.prefix_state + (size_t)c * stride
+                                     : t.own_state + (size_t)(c - prefix_chunks) * t.own_stride);
+}
+
 // The running sums of a row's states c = first, first + G, ...: `B` of them on their way at a time.
-// base: state row 0 of the row's kv head, and the head in the group.
 template <int D, int G, int B>
 __device__ __forceinline__ void join_states(const BatchArgs &a, const BatchToken &t, size_t base, int prefix_chunks,
                                             int stride, int first, int n, int d, float &m, float &l, f32x4 &acc) {
@@ -801,9 +832,7 @@ __device__ __forceinline__ void join_states(const BatchArgs &a, const BatchToken
         float mm[B], ll[B], top = m;
 #pragma unroll
         for (int b = 0; b < B; b++) {
-            const int c = min(c0 + b * G, n - 1);
-            const size_t at = base + (c < prefix_chunks ? t.prefix_state + (size_t)c * stride
-                                                        : t.own_state + (size_t)(c - prefix_chunks) * t.own_stride);
+            const size_t at = state_of(t, base, prefix_chunks, stride, min(c0 + b * G, n - 1));
             o[b] = *reinterpret_cast<const f32x4 *>(a.po + at * D + d);
             mm[b] = a.pm[at];
             ll[b] = a.pl[at];
@@ -818,10 +847,30 @@ __device__ __forceinline__ void join_states(const BatchArgs &a, const BatchToken
         for (int b = 0; b < B; b++)
             if (c0 + b * G < n) {
                 const float f = exp2f(mm[b] - top);
-                l += f * ll[b];
-                acc += f * o[b];
+                l += f * fabsf(ll[b]);
+                acc += (ll[b] < 0.0f ? f / kLow : f) * o[b];
             }
     }
+}
+
+// The values of a row's `mean` again whose sum overflowed, from sums at 2^-32, state after state.
+__device__ __forceinline__ f32x4 join_low(const BatchArgs &a, const BatchToken &t, size_t base, int prefix_chunks,
+                                          int stride, int n, int D, int d, f32x4 sum, f32x4 mean) {
+    float top = kNoMax, l = 0.0f;
+    f32x4 low{};
+    for (int c = 0; c < n; c++) top = fmaxf(top, a.pm[state_of(t, base, prefix_chunks, stride, c)]);
+    for (int c = 0; c < n; c++) {
+        const size_t at = state_of(t, base, prefix_chunks, stride, c);
+        const float f = exp2f(a.pm[at] - top), ll = a.pl[at];
+        l += f * kLow * fabsf(ll);
+        low += (ll < 0.0f ? f : f * kLow) * *reinterpret_cast<const f32x4 *>(a.po + at * D + d);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) mean[e] = mean_of(sum[e], mean[e], low[e], l);
+    return mean;
+}
+__device__ __forceinline__ bool finite(f32x4 x) {
+    return fabsf(x[0]) < INFINITY && fabsf(x[1]) < INFINITY && fabsf(x[2]) < INFINITY && fabsf(x[3]) < INFINITY;
 }
 
 // W waves join one row's states: with the largest m, weights 2^(m_i - m), att = sum w O /
@@ -884,9 +933,11 @@ __global__ __launch_bounds__(256) void batch_merge_kernel(BatchArgs a) {
             }
             __syncthreads();
         }
-        f = 1.0f / l;
-        if (lane < L && (W == 1 || wave == 0))
-            *reinterpret_cast<f32x4 *>(a.att + ((size_t)t.merge * heads + head) * D + d) = acc * f;
+        if (lane < L && (W == 1 || wave == 0)) {
+            f32x4 y = acc * (1.0f / l);
+            if (!finite(acc)) y = join_low(a, t, base, prefix_chunks, stride, n, D, d, acc, y);
+            *reinterpret_cast<f32x4 *>(a.att + ((size_t)t.merge * heads + head) * D + d) = y;
+        }
     }
 }
 
@@ -902,11 +953,14 @@ __global__ __launch_bounds__(256) void batch_merge_rows_kernel(BatchArgs a) {
     for (int w = blockIdx.x * R + threadIdx.x / L; w < work; w += gridDim.x * R) {
         const int i = divide(w, heads, a.inv_heads), head = w - i * heads, kh = divide(head, a.group, a.inv_group);
         const BatchToken t = a.tokens[i];
+        const size_t base = (size_t)kh * a.state_rows + (head - kh * a.group);
+        const int n = prefix_chunks + t.own_chunks;
         float m = kNoMax, l = 0.0f;
         f32x4 acc{};
-        join_states<D, 1, 4>(a, t, (size_t)kh * a.state_rows + (head - kh * a.group), prefix_chunks, stride, 0,
-                             prefix_chunks + t.own_chunks, d, m, l, acc);
-        *reinterpret_cast<f32x4 *>(a.att + ((size_t)t.merge * heads + head) * D + d) = acc * (1.0f / l);
+        join_states<D, 1, 4>(a, t, base, prefix_chunks, stride, 0, n, d, m, l, acc);
+        f32x4 y = acc * (1.0f / l);
+        if (!finite(acc)) y = join_low(a, t, base, prefix_chunks, stride, n, D, d, acc, y);
+        *reinterpret_cast<f32x4 *>(a.att + ((size_t)t.merge * heads + head) * D + d) = y;
     }
 }
 
