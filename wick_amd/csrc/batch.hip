@@ -797,7 +797,8 @@ __global__ __launch_bounds__(256, 2) void batch_attend_kernel(BatchArgs a) {
 #pragma unroll
             for (int e = 0; e < E; e++) acc[e] += f * j.o[i][row][d0 + e];
         }
-        bool odd = !(fabsf(sum) < INFINITY) || (sum == 0.0f && (it.p1 > it.p0 || last_of(row) >= it.o0));
+        bool odd = !(fabsf(sum) < INFINITY);
+        if (__any(sum == 0.0f)) odd |= sum == 0.0f && (it.p1 > it.p0 || last_of(row) >= it.o0);
 #pragma unroll
         for (int e = 0; e < E; e++) odd |= !(fabsf(acc[e]) < INFINITY);
         if (odd && row < it.nrows) j.redo[row] = 1;
