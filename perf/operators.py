@@ -224,7 +224,10 @@ def _batch(s):
 
 def prepare(case, seed):
     if case["kind"] == "logits":
-        return _logits_inputs(case, seed)
+        s = _logits_inputs(case, seed)
+        if own:  # the program's stream does not wait for the one that makes the inputs
+            torch.cuda.synchronize()
+        return s
     s = _attention_inputs(case, seed)
     s["att"] = torch.empty_like(s["q"])
     if own:
