@@ -26,6 +26,12 @@ static int check(BatchLimits c, const std::vector<int> &start, const std::vector
     c.max_tokens = std::max(1, total) + spare;
     const BatchPlan p = batch_plan(c, start.data(), t.data(), prefix);
     const char *what = nullptr;
+    // the smallest handle that takes the step
+    BatchLimits tight = c;
+    tight.prefix_capacity = prefix;
+    tight.capacity = 1;
+    for (size_t i = 0; i < t.size(); i++) tight.capacity = std::max(tight.capacity, start[i] + t[i]);
+    if (p.state_rows > batch_max_state_rows(tight)) what = "more state rows than the smallest handle holds";
     if (p.head.items != (int)p.items.size()) what = "item count";
     if (p.head.items > batch_max_items(c)) what = "more items than a handle holds";
     if (p.head.items > p.head.most_items) what = "more items than a captured call launches";
@@ -68,6 +74,16 @@ int main(int argc, char **argv) {
         bad += check(limits(3, 3, bf16), {0, 100, 100, 100}, {40, 1, 1, 1}, 32768, 0);
         bad += check(limits(8, 4, bf16), {0, 100, 100}, {15, 1, 1}, 32768, 5000);
         bad += check(limits(7, 2, bf16), {0, 100, 100, 100}, {16, 1, 1, 1}, 60000, 5000);
+    }
+    // a handle holds states for its own rows and positions: four tokens of three rows against up to three
+    // ranges of 300 prefix positions and one of 61
+    BatchLimits four = limits(3, 3, false);
+    four.sequences = four.max_tokens = 4;
+    four.capacity = 61;
+    four.prefix_capacity = 300;
+    if (batch_max_state_rows(four) > 4 * 3 * (3 + 1)) {
+        std::printf("%lld state rows for four tokens\n", (long long)batch_max_state_rows(four));
+        bad++;
     }
     auto pick = [&](int lo, int hi) { return (int)(lo + g() % (unsigned)(hi - lo + 1)); };
     auto spread = [&](int lo, int hi) {  // over the logarithm, lo >= 1

@@ -95,7 +95,10 @@ inline int64_t batch_max_state_rows(const BatchLimits &c) {
     const int64_t rows = (int64_t)c.max_tokens * c.group, few = std::min(c.sequences, c.max_tokens);
     const int64_t slots = c.cus / c.kv_heads + 1;
     const int64_t split = std::min(rows, 3 * kBatchWide * slots + (kBatchFew + kBatchWide) * few);
-    return 6 * kBatchWide * slots + 2 * split + 2 * kBatchWide;
+    // the least range is kBatchStep keys for either kind of block (kPlanLeastWide, kPlanLeastNarrow)
+    auto ranges_of = [](int64_t keys) { return (keys + kBatchStep - 1) / kBatchStep; };
+    const int64_t ranges = ranges_of(c.prefix_capacity) + ranges_of(c.capacity);
+    return std::min(6 * kBatchWide * slots + 2 * split + 2 * kBatchWide, rows * ranges);
 }
 
 struct BatchPlan {
@@ -113,6 +116,7 @@ constexpr double kPlanItem = 2.0;  // an item's cost besides its keys'
 // (32/8 heads, bf16): 158 whole, 174 split.
 constexpr double kPlanJoin = 18.0, kPlanLone = 1.3;
 constexpr double kPlanLeastWide = 4.0, kPlanLeastNarrow = 1.0;  // least cost of a range of keys
+static_assert(32 * kPlanLeastWide == kBatchStep && 128 * kPlanLeastNarrow == kBatchStep, "batch_max_state_rows counts on it");
 // Ranges up to which small sequences are not cut, to save the second launch: four tokens behind a
 // prefix of 100 (9/3 heads of 64) 6.8 us, cut 9.0; of 200 8.2 and 9.2; of 300 9.5 and 9.3.
 constexpr double kPlanAlone = 1.6;
