@@ -1,8 +1,10 @@
 """Steps of a batch that mix prompts and single tokens behind a long prefix, run and captured, against
 64-bit arithmetic under the tolerances of test_batch_gpu."""
+import numpy as np
 import pytest
 import torch
 
+from wick_amd.batch import DeviceBatch
 from test_batch_gpu import DEV, U, Case
 
 pytestmark = pytest.mark.gpu
@@ -51,3 +53,36 @@ def test_captured_beside_single_tokens(heads, kv_heads, d, start, t, prefix):
                 # the graph's join may sum in another order: each of two sums over at most n = 200
                 # states is off by (n + 4) u of the largest value, below 6 here
                 assert float((att - c.run()).abs().max()) < 2 * 204 * U * 6, i
+
+
+def test_steps_beside_another_handles_capture():
+    """Plans and steps of one handle while another's are captured: neither disturbs the other."""
+    a, b = (Case(8, 2, 64, [50, 3], [1, 20], 400, seed=40 + i).fill() for i in range(2))
+    wants = [a.check(), b.check()]
+    att = torch.zeros_like(wants[1])
+    out = torch.zeros_like(wants[0])
+    q = a.q.cpu().numpy()
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    b.b.set_stream(stream.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        b.b.attention_device(0, b.q.data_ptr(), att.data_ptr())
+        for _ in range(3):
+            a.b.plan(a.start, a.t, a.prefix)
+            a.b.attention_device(0, a.q.data_ptr(), out.data_ptr())
+        a.b.synchronize()
+        host = a.b.attention(0, q)
+        with DeviceBatch(1, 8, 2, 64, 1, 4) as other:
+            other.plan([0], [2])
+            other.append(0, np.ones((2, 128), np.float32), np.full((2, 128), 3, np.float32))
+            k, v = other.read(0, 0, 0, 2)
+            assert (k == 1).all() and (v == 3).all()
+    torch.cuda.synchronize()
+    assert torch.equal(out, wants[0]) and torch.equal(torch.from_numpy(host).to(DEV), wants[0])
+    for _ in range(3):
+        with torch.cuda.stream(stream):
+            att.zero_()
+            graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(att, wants[1])

@@ -101,6 +101,20 @@ class OnDevice {
     OnDevice on_((b)->device); \
     if (on_.rc != hipSuccess) return hip_fail(on_.rc, "hipSetDevice")
 
+// For the length of a call: what it waits for or allocates would, in the default mode, end a
+// capture in progress on another handle's or program's stream.
+class BesideCaptures {
+  public:
+    BesideCaptures() { changed_ = hipThreadExchangeStreamCaptureMode(&mode_) == hipSuccess; }
+    ~BesideCaptures() {
+        if (changed_) (void)hipThreadExchangeStreamCaptureMode(&mode_);
+    }
+
+  private:
+    hipStreamCaptureMode mode_ = hipStreamCaptureModeRelaxed;
+    bool changed_;
+};
+
 bool capturing(hipStream_t s) {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
     if (hipStreamIsCapturing(s, &st) != hipSuccess) {
@@ -233,6 +247,7 @@ int wick_hip_batch_create(const wick_hip_batch_config *cfg, wick_hip_batch **out
     if (!cfg || !out) return set_error(WICK_HIP_EINVAL, "null argument");
     *out = nullptr;
     if (int rc = check_config(*cfg)) return rc;
+    BesideCaptures beside;
     int ndev = 0;
     if (hipGetDeviceCount(&ndev) != hipSuccess || ndev < 1) return set_error(WICK_HIP_EDEVICE, "no HIP device");
     wick_hip_batch *b = new (std::nothrow) wick_hip_batch;
@@ -255,6 +270,7 @@ int wick_hip_batch_create(const wick_hip_batch_config *cfg, wick_hip_batch **out
 void wick_hip_batch_destroy(wick_hip_batch *b) {
     if (!b) return;
     OnDevice on(b->device);
+    BesideCaptures beside;
     if (b->stream) (void)hipStreamSynchronize(b->stream);
     for (void *p : {(void *)b->pk, (void *)b->pv, (void *)b->k, (void *)b->v, (void *)b->plan_dev, (void *)b->states,
                     (void *)b->stage})
@@ -285,6 +301,7 @@ int wick_hip_batch_load_prefix(wick_hip_batch *b, const wick_hip_kv *kv, int len
     wick::kv_layer(kv, 0, &k, &v, &device);
     if (device != b->device) return set_error(WICK_HIP_EINVAL, "the cache is on device %d, the batch on %d", device, b->device);
     ON_DEVICE(b);
+    BesideCaptures beside;
     if (capturing(b->stream) || capturing(info.stream))
         return set_error(WICK_HIP_EINVAL, "wick_hip_batch_load_prefix on a stream that is being captured");
     HIP_TRY(hipStreamSynchronize(info.stream));
@@ -338,6 +355,7 @@ int wick_hip_batch_plan(wick_hip_batch *b, const int *start, const int *t, int p
     if (total > c.max_tokens)
         return set_error(WICK_HIP_EINVAL, "%lld tokens exceed max_tokens %d", total, c.max_tokens);
     ON_DEVICE(b);
+    BesideCaptures beside;
     if (capturing(b->stream)) return set_error(WICK_HIP_EINVAL, "wick_hip_batch_plan on a stream that is being captured");
     try {
         wick::BatchPlan p = wick::batch_plan(b->lim, start, t, prefix);
@@ -451,6 +469,7 @@ int wick_hip_batch_append(wick_hip_batch *b, int layer, const float *k, const fl
     if (b->head.total == 0) return WICK_HIP_OK;
     if (!k || !v) return set_error(WICK_HIP_EINVAL, "null k or v");
     ON_DEVICE(b);
+    BesideCaptures beside;
     const size_t n = (size_t)b->head.total * b->cfg.kv_heads * b->cfg.head_dim;
     if (int rc = stage_for(b, 2 * n)) return rc;
     HIP_TRY(hipMemcpyAsync(b->stage, k, n * sizeof(float), hipMemcpyHostToDevice, b->stream));
@@ -466,6 +485,7 @@ int wick_hip_batch_attention(wick_hip_batch *b, int layer, const float *q, float
     if (b->head.total == 0) return WICK_HIP_OK;
     if (!q || !att) return set_error(WICK_HIP_EINVAL, "null q or att");
     ON_DEVICE(b);
+    BesideCaptures beside;
     const size_t n = (size_t)b->head.total * b->cfg.heads * b->cfg.head_dim;
     if (int rc = stage_for(b, 2 * n)) return rc;
     HIP_TRY(hipMemcpyAsync(b->stage, q, n * sizeof(float), hipMemcpyHostToDevice, b->stream));
@@ -484,6 +504,7 @@ int wick_hip_batch_read(wick_hip_batch *b, int layer, int seq, int pos0, int n, 
     if (n < 1 || pos0 < 0 || (long long)pos0 + n > capacity)
         return set_error(WICK_HIP_EINVAL, "positions %d..%lld exceed the capacity %d", pos0, (long long)pos0 + n, capacity);
     ON_DEVICE(b);
+    BesideCaptures beside;
     const size_t floats = (size_t)n * c.kv_heads * c.head_dim;
     if (int rc = stage_for(b, floats)) return rc;
     for (int x = 0; x < 2; x++) {
@@ -515,6 +536,7 @@ int wick_hip_batch_set_stream(wick_hip_batch *b, void *stream) {
 int wick_hip_batch_synchronize(wick_hip_batch *b) {
     if (!b) return set_error(WICK_HIP_EINVAL, "null batch handle");
     ON_DEVICE(b);
+    BesideCaptures beside;
     HIP_TRY(hipStreamSynchronize(b->stream));
     return WICK_HIP_OK;
 }
