@@ -30,10 +30,13 @@ extern "C" int wick_hip_logits_adjust_device(const wick_hip_logit_rules *rules, 
                           (const void *)r.bias, (const void *)r.mask, (const void *)r.mask_row})
         if (reinterpret_cast<uintptr_t>(p) & 3u) return set_error(WICK_HIP_EINVAL, "an array is not 4-byte aligned");
     if (rows == 0) return WICK_HIP_OK;
-    // in place, or apart: a workgroup reads its own ids only
+    // in place, or apart (in memory, or with every row of one between two of the other): a workgroup reads its
+    // own ids only
     const uintptr_t x0 = reinterpret_cast<uintptr_t>(logits), y0 = reinterpret_cast<uintptr_t>(out);
     const uintptr_t x1 = x0 + ((size_t)(rows - 1) * stride + vocab) * 4, y1 = y0 + ((size_t)(rows - 1) * out_stride + vocab) * 4;
-    if (x0 < y1 && y0 < x1 && !(x0 == y0 && (stride == out_stride || rows == 1)))
+    const size_t at = (y0 > x0 ? y0 - x0 : x0 - y0) / 4 % stride;  // of a row behind the other's before it
+    const bool between = stride == out_stride && at >= (size_t)vocab && at <= (size_t)(stride - vocab);
+    if (x0 < y1 && y0 < x1 && !between && !(x0 == y0 && (stride == out_stride || rows == 1)))
         return set_error(WICK_HIP_EINVAL, "out overlaps logits");
     wick::LogitArgs a{};
     a.r = r;
