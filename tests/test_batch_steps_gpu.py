@@ -86,3 +86,37 @@ def test_steps_beside_another_handles_capture():
             graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(att, wants[1])
+
+
+@pytest.mark.parametrize("heads,kv_heads,d,start,t,prefix", [
+    (200, 1, 16, [0, 7], [3, 1], 200),       # a token's rows fill more than one item
+    (257, 1, 32, [0, 30], [9, 2], 3000),
+    (64, 64, 16, [0, 5, 0], [70, 1, 0], 150),
+    (512, 2, 64, [40], [1], 9000),
+])
+def test_many_heads(heads, kv_heads, d, start, t, prefix):
+    Case(heads, kv_heads, d, start, t, prefix, seed=heads).fill().check()
+
+
+def test_many_sequences():
+    """Most of them bring nothing, the others one token or a few."""
+    rng = np.random.default_rng(5)
+    t = [int(x) for x in rng.choice([0, 0, 0, 1, 1, 3], 1500)]
+    Case(6, 2, 32, [int(x) for x in rng.integers(0, 9, 1500)], t, 700, seed=5).fill().check()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("heads,kv_heads,d,start,t,prefix", [
+    (8, 2, 64, [0, 40], [9, 1], 0),
+    (32, 8, 128, [0, 40, 3], [200, 1, 1], 2500),
+])
+def test_a_padding_row_of_queries(heads, kv_heads, d, start, t, prefix, bad):
+    """Queries of one token that are no numbers: its result is none, the others' are as they were."""
+    c = Case(heads, kv_heads, d, start, t, prefix, seed=60).fill()
+    want, tol = c.want()
+    q = c.q.clone()
+    q[3] = bad
+    got = c.run(q)
+    assert not bool(torch.isfinite(got[3]).any())
+    rest = torch.arange(len(got), device=DEV) != 3
+    assert bool(((got.double() - want).abs() <= tol)[rest].all())
