@@ -111,9 +111,10 @@ struct BatchPlan {
 // The constants of the plan, in tiles of 32 keys by a wide item (about 2 us at head_dim 128).
 constexpr double kPlanItem = 2.0;  // an item's cost besides its keys'
 // What leaving states and joining them costs a step, and what a tile of a lone wide item on a
-// unit takes against one of two.  16 prompts of 13..161 tokens behind a prefix of 1500 (16/8 heads
-// of 128): split 98 us, whole 128; one prompt of 512: 29.5 and 43.8; six prompts of 697..2047
-// (32/8 heads, bf16): 158 whole, 174 split.
+// unit takes against one of two.  16 prompts of 12..161 tokens behind a prefix of 1500 (16/8 heads
+// of 128): split 105 us, whole 128; one prompt of 512: 28.3 and 43.7; of 1000 (32/8 of 128) 74 and 79, but
+// 56 and 47 on a bf16 cache; of 2000 (14/2 of 64) 62 and 78.  Eight prompts of 33..701 (14/2 of 64) with a
+// price of 0, 6, 12 and 18: 38.3, 37.4, 39.9 and 37.1.
 constexpr double kPlanJoin = 18.0, kPlanLone = 1.3;
 constexpr double kPlanLeastWide = 4.0, kPlanLeastNarrow = 1.0;  // least cost of a range of keys
 static_assert(32 * kPlanLeastWide == kBatchStep && 128 * kPlanLeastNarrow == kBatchStep, "batch_max_state_rows counts on it");

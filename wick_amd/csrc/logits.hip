@@ -5,9 +5,10 @@
 // the same counts) and applies the penalties, notes each id's last bias there and adds
 // them, then writes its part of the row.  A row's tokens are read once per slab, from the L2.
 //
-// Bound: HBM, 8 bytes a logit and a mask bit: 64 rows of 128256 with 1500 tokens each 14.2 us, 4.7 TB/s
-// (a copy of as many bytes 10.1); one row of 49152 is the launch (3 us on the GPU).  One LDS word an
-// id, used for the counts and then for the biases: with a word for each the 64 rows took 18.1.
+// Bound: 8 bytes a logit and a mask bit, and the dependent reads and barriers of a workgroup (n_tokens, tokens,
+// the row's settings, biases): 64 rows of 128256 with 1500 tokens each 14.2 us, where a copy of as many
+// bytes, which the last-level cache holds like these, takes 10.1; one row of 49152 is the launch (3 us on the GPU).
+// One LDS word an id, used for the counts and then for the biases: with a word for each the 64 rows took 18.1.
 #include <hip/hip_runtime.h>
 
 #include "logits_kernels.h"
