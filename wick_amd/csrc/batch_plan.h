@@ -206,8 +206,8 @@ inline BatchPlan batch_plan(const BatchLimits &c, const int *start, const int *t
         }
     // What a range should cost.  Split big sequences make the blocks of all split rows wide: there the
     // other sequences' few rows add up to a wide block, not the narrow ones of a step of their own.
-    const double cost = with_shared(shared_of(alone ? small_rows : split_rows)) * c.kv_heads / c.cus;
-    const double target = wides ? cost / kPlanWideItems : cost;
+    const double cut = with_shared(shared_of(alone ? small_rows : split_rows)) * c.kv_heads / c.cus;
+    const double target = wides ? cut / kPlanWideItems : cut;
 
     // n even ranges over the keys of a block, each near the target, in steps
     auto range = [&](int block, int keys) {
